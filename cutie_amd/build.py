@@ -13,7 +13,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcutie_hip.so")
 SOURCES = ["core.hip", "grid_build.hip", "embed.hip", "norm.hip", "loss.hip", "optim.hip", "conv_mfma.hip", "conv_wide.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
+         # no packed f32 instructions (v_pk_add_f32 and the like): some of their forms have given wrong results on gfx950
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(out, deps):
