@@ -374,6 +374,75 @@ def spatial_mean_bcast(x, out, scratch=None):
     return out
 
 
+# ------------------------------------------------------------------------------------ K15
+GN_EPS = 1e-5
+GN_ACTIVATION_CODE = dict(ACTIVATION_CODE, silu=3)
+
+
+def _f32_vec(t, n, device, what):
+    """an optional contiguous f32 vector of n elements on `device`"""
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous() or t.device != device):
+        raise capi.CutieError("%s must be a contiguous f32 tensor of %d elements on %s" % (what, n, device))
+    return t
+
+
+def _workspace(workspace, need, device, what):
+    if workspace is None:
+        return torch.empty(max(int(need), 16), dtype=torch.uint8, device=device)
+    if workspace.device != device or not workspace.is_contiguous():
+        raise capi.CutieError("%s: the workspace must be a contiguous tensor on %s" % (what, device))
+    return workspace
+
+
+def gn_workspace_bytes(B, HW, C, groups):
+    return capi.lib().cutie_gn_workspace_bytes(int(B), int(HW), int(C), int(groups))
+
+
+def _gn_views(what, x, stats, act, others):
+    if x.dim() != 4 or stats.dim() != 3 or stats.shape[0] != x.shape[0] or stats.shape[2] != 2:
+        raise capi.CutieError("%s: x is [B,H,W,C] and stats [B,groups,2], got %s and %s" % (what, tuple(x.shape), tuple(stats.shape)))
+    if act not in GN_ACTIVATION_CODE:
+        raise capi.CutieError("%s: unknown activation %r (none, relu, sigmoid, silu)" % (what, act))
+    if stats.dtype != torch.float32 or not stats.is_contiguous() or stats.device != x.device:
+        raise capi.CutieError("%s: stats must be contiguous f32 on %s" % (what, x.device))
+    for t in others:
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+            raise capi.CutieError("%s: views differ: %s %s against %s %s" % (what, tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
+    return _bhwc(x)
+
+
+def _gn_ld(t):
+    """ld_of, also for views with a dimension of one (their strides say nothing)"""
+    return ld_of(t) if t.shape[1] * t.shape[2] and t.shape[0] else t.shape[3]
+
+
+def gn_fwd(x, y, stats, gamma=None, beta=None, act=None, eps=GN_EPS, workspace=None):
+    """Group norm with an activation (cutie_gn_fwd): y = act(gamma * (x - mean) * rstd + beta) over the C / groups channels and
+    all pixels of a (sample, group).  x, y [B,H,W,C] views of one element type; stats f32 [B,groups,2] receives (mean, rstd) for
+    gn_bwd; gamma / beta f32 [C] or None; act None, 'relu', 'sigmoid' or 'silu'.  workspace: optional uint8 tensor of
+    gn_workspace_bytes(B, H*W, C, groups) bytes.  Returns y."""
+    B, HW, C = _gn_views("gn_fwd", x, stats, act, (y,))
+    need = gn_workspace_bytes(B, HW, C, stats.shape[1])
+    ws = _workspace(workspace, need, x.device, "gn_fwd")
+    call("cutie_gn_fwd", ptr(x), _gn_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_fwd: gamma")),
+         ptr(_f32_vec(beta, C, x.device, "gn_fwd: beta")), stats.shape[1], float(eps), GN_ACTIVATION_CODE[act], ptr(y), _gn_ld(y),
+         dt_of(x), ptr(stats), B, HW, C, ptr(ws), ws.numel() * ws.element_size(), stream())
+    return y
+
+
+def gn_bwd(dy, x, stats, dx, gamma=None, beta=None, act=None, dgamma=None, dbeta=None, accumulate=False, workspace=None):
+    """Gradient of gn_fwd (cutie_gn_bwd): x and stats of the forward, the same gamma / beta / act; dx [B,H,W,C] view; dgamma,
+    dbeta f32 [C] or None, overwritten or (accumulate) added to.  Returns dx."""
+    B, HW, C = _gn_views("gn_bwd", x, stats, act, (dy, dx))
+    need = gn_workspace_bytes(B, HW, C, stats.shape[1])
+    ws = _workspace(workspace, need, x.device, "gn_bwd")
+    call("cutie_gn_bwd", ptr(dy), _gn_ld(dy), ptr(x), _gn_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_bwd: gamma")),
+         ptr(_f32_vec(beta, C, x.device, "gn_bwd: beta")), stats.shape[1], GN_ACTIVATION_CODE[act], ptr(stats), ptr(dx), _gn_ld(dx),
+         dt_of(x), ptr(_f32_vec(dgamma, C, x.device, "gn_bwd: dgamma")), ptr(_f32_vec(dbeta, C, x.device, "gn_bwd: dbeta")),
+         1 if accumulate else 0, B, HW, C, ptr(ws), ws.numel() * ws.element_size(), stream())
+    return dx
+
+
 # ------------------------------------------------------------------------------------ K9-K11
 def softmax_ce_fwd(logits, labels, C, ce, probs, bad):
     """logits [..., >=C] view; labels int32 [...]; ce f32 [N]; probs f32 [N,C] or None."""

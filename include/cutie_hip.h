@@ -331,6 +331,31 @@ int cutie_spatial_mean_bcast(const void* x, int ld_x, int x_dtype, void* out, in
                              cutie_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * K15  group norm with an activation, channels last.   No counterpart in the reference, whose only norm is K6's instance
+ *     norm (model_framework.py:423); for layers whose statistics should not depend on one channel's plane alone.
+ * A group is C / groups consecutive channels of a sample, N = HW * C / groups values; biased variance:
+ *   fwd: mean, rstd = 1/sqrt(var + eps) of each (sample, group) -> stats f32 [B][groups][2];
+ *        y = act(gamma[c] * (x - mean) * rstd + beta[c]),  act: 0 none, 1 ReLU, 2 sigmoid, 3 SiLU (CUTIE_ACT_SILU)
+ *   bwd: with g = dy * act'(gamma * xhat + beta), xhat = (x - mean) * rstd from the stats of the forward:
+ *        dx = rstd * (g*gamma - mean_N(g*gamma) - xhat * mean_N(g*gamma*xhat)),
+ *        dgamma[c] = sum g * xhat, dbeta[c] = sum g over (b, hw)  (each nullable; accumulate != 0 adds to what is there)
+ * gamma / beta f32 [C], each nullable (1 and 0).  x, y, dy, dx share one dtype, any channel count that `groups` divides, any
+ * leading dimension >= C; views whose base, leading dimension and group width are multiples of 16 bytes move fastest.
+ * An output may not overlap an input (slices of one wide buffer are fine).  Sums are f32 or f64 in a fixed order: reruns are bit-identical.  A value next to the
+ * step of the ReLU takes the side that f64 arithmetic on (x, stats, gamma, beta) gives.  B, C, groups <= 65535, eps > 0.
+ * workspace: cutie_gn_workspace_bytes(B, HW, C, groups) bytes, 16-byte aligned, clobbered, no pre-fill.  B = 0 or HW = 0
+ * stores no activations; dgamma and dbeta are then cleared (accumulate == 0) or left alone. */
+#define CUTIE_ACT_SILU 3
+size_t cutie_gn_workspace_bytes(int B, int HW, int C, int groups);
+int cutie_gn_fwd(const void* x, int ld_x, const float* gamma /* nullable */, const float* beta /* nullable */, int groups,
+                 float eps, int act, void* y, int ld_y, int dtype, float* stats, int B, int HW, int C,
+                 void* workspace, size_t workspace_bytes, cutie_stream_t stream);
+int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, const float* gamma /* nullable */,
+                 const float* beta /* nullable */, int groups, int act, const float* stats, void* dx, int ld_dx, int dtype,
+                 float* dgamma /* nullable */, float* dbeta /* nullable */, int accumulate, int B, int HW, int C,
+                 void* workspace, size_t workspace_bytes, cutie_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * K9-K11  per-cell softmax cross-entropy with hard negative mining.   Replaces
  *     Model.softmax (model_framework.py:318-320) and CUTIE.build_loss
  *     (model_cutie.py:107-130; duplicate at model_cutie2.py:114-147).
