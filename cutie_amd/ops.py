@@ -73,6 +73,53 @@ def embed_bwd(ids, dout, dtable, workspace=None):
     return dtable
 
 
+# ------------------------------------------------------------------------------------ K16
+def _rows_ld(t):
+    """leading dimension of a [..., E] view whose leading axes collapse to one row index"""
+    return ld_of(t) if t.dim() > 1 and t.numel() else t.shape[-1]
+
+
+def _check_ids(what, ids, rows, table):
+    V, E = table.shape
+    if ids.dtype != torch.int32 or not ids.is_contiguous():
+        raise capi.CutieError("%s: ids must be contiguous int32" % what)
+    if table.dtype != torch.float32 or not table.is_contiguous():
+        raise capi.CutieError("%s: the table must be contiguous f32 [V,E]" % what)
+    if rows.shape[-1] != E or rows.numel() != ids.numel() * E:
+        raise capi.CutieError("%s: rows %s do not match %d ids of E=%d" % (what, tuple(rows.shape), ids.numel(), E))
+    if ids.device != rows.device or table.device != rows.device:
+        raise capi.CutieError("%s: tensors on different devices" % what)
+
+
+def embed_scaled_fwd(ids, table, out, scale, oob):
+    """out[cell] = scale * table[ids[cell]] (cutie_embed_scaled_fwd): ids int32 [...]; table f32 [V,E], any E; out [...,E] view;
+    oob int32 [1] counter of ids outside [0,V) (their rows are zero).  Returns out."""
+    _check_ids("embed_scaled_fwd", ids, out, table)
+    if oob.dtype != torch.int32 or oob.device != out.device:
+        raise capi.CutieError("embed_scaled_fwd: oob must be int32 on %s" % out.device)
+    V, E = table.shape
+    call("cutie_embed_scaled_fwd", ptr(ids), ids.numel(), ptr(table), V, E, float(scale), ptr(out), _rows_ld(out), dt_of(out),
+         ptr(oob), stream())
+    return out
+
+
+def embed_grad_sorted_workspace_bytes(n_cells, V, E):
+    return capi.lib().cutie_embed_grad_sorted_workspace_bytes(int(n_cells), int(V), int(E))
+
+
+def embed_grad_sorted(ids, dout, dtable, scale=1.0, accumulate=False, workspace=None):
+    """dtable[v] = scale * sum of dout rows whose id is v, over cells sorted by id (cutie_embed_grad_sorted): the same bits every
+    run, whatever the ids repeat.  accumulate: add to dtable instead of storing all of its rows.  workspace: optional uint8 tensor
+    of embed_grad_sorted_workspace_bytes(n, V, E) bytes.  Returns dtable."""
+    _check_ids("embed_grad_sorted", ids, dout, dtable)
+    V, E = dtable.shape
+    n = ids.numel()
+    ws = _workspace(workspace, embed_grad_sorted_workspace_bytes(n, V, E), dout.device, "embed_grad_sorted")
+    call("cutie_embed_grad_sorted", ptr(ids), n, ptr(dout), _rows_ld(dout), dt_of(dout), float(scale), ptr(dtable), V, E,
+         1 if accumulate else 0, ptr(ws), ws.numel() * ws.element_size(), stream())
+    return dtable
+
+
 # ------------------------------------------------------------------------------------ K2-K5
 def wgrad_descs(tasks):
     """tasks: list of (x view [B,H,W,>=cin], cin, dz view [B,H,W,>=cout], cout, kh, kw, dil, dw f32 [kh,kw,cin,cout],

@@ -104,6 +104,24 @@ int cutie_embed_bwd(const int32_t* ids, int64_t n_cells, const void* dout, int l
                     void* workspace, size_t workspace_bytes, cutie_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * K16  embedding lookup with a scale, and its gradient by sorted tokens.   No counterpart in the reference, which neither
+ *     scales its rows nor fixes the order in which tf.gradients adds them (Model.embed, model_framework.py:43-54).
+ * fwd:  out[cell, 0:E] = scale * table[ids[cell], 0:E], any E; an id outside [0, V) gives a zero row and bumps *oob_count, as
+ *       K1.  One rounding to out_dtype, from the f32 product.
+ * grad: dtable[v, 0:E] = scale * (sum of dout[cell, 0:E] over ids[cell] == v); accumulate == 0 stores every row of dtable
+ *       (zeros where no cell has the id), else the sums are added to what is there and other rows are left alone.  An id
+ *       outside [0, V) adds to nothing.  The cells are ordered by a stable sort on the id and every row has one owner: f32
+ *       sums in an order that ids, V, E and the alignment of the views fix, no atomics, the same bits every run.
+ * E = 1 .. 65536, n_cells <= 2^30, V < 2^30; views whose base and leading dimension are multiples of 16 bytes move fastest.
+ * workspace: cutie_embed_grad_sorted_workspace_bytes(n_cells, V, E) bytes, 16-byte aligned, clobbered, no pre-fill. */
+int cutie_embed_scaled_fwd(const int32_t* ids, int64_t n_cells, const float* table, int V, int E, float scale,
+                           void* out, int ld_out, int out_dtype, int32_t* oob_count, cutie_stream_t stream);
+size_t cutie_embed_grad_sorted_workspace_bytes(int64_t n_cells, int V, int E);
+int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, const void* dout, int ld_dout, int dout_dtype, float scale,
+                            float* dtable, int V, int E, int accumulate, void* workspace, size_t workspace_bytes,
+                            cutie_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * K2-K5  stride-1 SAME (dilated) cross-correlation as an implicit GEMM on MFMA, with the
  *     bias + ReLU epilogue and the instance-norm statistics.   Replaces tf.nn.conv2d /
  *     tf.nn.atrous_conv2d + bias_add + relu in Model.conv / dilate_conv / convolution,
