@@ -11,7 +11,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcutie_hip.so")
-SOURCES = ["core.hip", "grid_build.hip", "embed.hip", "embed_sorted.hip", "norm.hip", "group_norm.hip", "loss.hip", "optim.hip", "conv_mfma.hip", "conv_wide.hip"]
+SOURCES = ["core.hip", "grid_build.hip", "embed.hip", "embed_sorted.hip", "norm.hip", "group_norm.hip", "loss.hip", "optim.hip", "muon.hip", "conv_mfma.hip", "conv_wide.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
          # no packed f32 instructions (v_pk_add_f32 and the like): some of their forms have given wrong results on gfx950

@@ -48,6 +48,15 @@ class SumRowsDesc(ctypes.Structure):
     _fields_ = [("part", ctypes.c_void_p), ("out", ctypes.c_void_p), ("C", ctypes.c_int)]
 
 
+class OrthDesc(ctypes.Structure):
+    _fields_ = [("g", ctypes.c_void_p), ("out", ctypes.c_void_p), ("rows", ctypes.c_int), ("cols", ctypes.c_int)]
+
+
+class MuonDesc(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("p_out", ctypes.c_void_p),
+                ("m_out", ctypes.c_void_p), ("rows", ctypes.c_int), ("cols", ctypes.c_int), ("out_scale", ctypes.c_float)]
+
+
 MAX_BATCH = 32
 POOL_TILES = 32
 
@@ -117,6 +126,9 @@ SIGNATURES = {
     "cutie_opt_norm": (_i, [_vp, _vp, _i64, _i64, _f, _vp, _i64, _i, _vp, _vp, _vp]),
     "cutie_opt_step": (_i, [_vp, _vp, _vp, _vp, _i64, _i64, _f, _f, _c.POINTER(PackDesc), _i, _i, _f, _f, _f, _f, _f, _f, _i,
                             _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "cutie_orthogonalize_workspace_bytes": (_sz, [_c.POINTER(_i), _i]),
+    "cutie_orthogonalize_batched": (_i, [_c.POINTER(OrthDesc), _i, _i, _f, _vp, _sz, _vp]),
+    "cutie_muon_step": (_i, [_c.POINTER(MuonDesc), _i, _f, _f, _i, _f, _f, _i, _f, _vp, _f, _f, _vp, _vp, _vp, _sz, _vp]),
     "cutie_batch_gather": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _i, _vp, _vp]),
     "cutie_batch_scatter_add": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp]),
     "cutie_convert": (_i, [_vp, _i, _i, _vp, _i, _i, _i64, _i, _vp]),

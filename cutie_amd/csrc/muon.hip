@@ -1,0 +1,634 @@
+// K17: the orthogonalised update.
+//
+//   X0 = U / (|U|_F + eps);   X <- X (a I + b A + c A A), A = X^T X   (steps times)
+// maps every singular value s of X0 to a s + b s^3 + c s^5, again and again: the quintic Newton-Schulz iteration with
+// a = 3.4445, b = -4.7750, c = 2.0315, which takes (0, 1] towards 1 (0.68 .. 1.21 after five steps from s >= 1e-2).  The update
+// around it: m' = mu m + g', U = g' + mu m' (or m'), p' = p (1 - lr wd) - lr k X.
+//
+// Number format.  Three products a step, all on the matrix cores, at f32 accuracy: a value v is held as two f16, hi = f16(v)
+// and lo = f16(v - hi), 22 significant bits, and a product is hi*hi + hi*lo + lo*hi with f32 accumulation (lo*lo is below the
+// 22 bits).  Against f64 the error is that of the f32 computation (2e-6 of the norm after five steps on a 256 x 1920 matrix in
+// both); one f16 or bf16 term instead gives 2e-2, since small singular values are amplified up to 3.4445 ** 5 = 485 times.
+// f16 has no range to spare, so each kind of matrix is kept at a fixed power of two: X (singular values at most 1.21)
+// times 2^12, A (at most 1.47) and B = b A + c A A (at most 2.81 in magnitude) times 2^13: entries stay below 23100, and
+// the smallest step of f16, 2^-24, is 2^-36 of X.
+//
+// Layout.  L = max(rows, cols) rows of S = min(rows, cols) values, both padded with zeros to multiples of 64 (the transpose of
+// a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
+// of a product is one 128-byte line of a row.  A and B [S][S] alike.
+#include "conv_common.h"
+
+namespace {
+using namespace cutie;
+using namespace cutie::convk;
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+constexpr float X_SCALE = 4096.f, INV_X_SCALE = 1.f / 4096.f;      // 2^12
+constexpr float AB_FROM_XX = 1.f / 2048.f;                         // 2^24 (X^T X) -> 2^13 A
+constexpr float AB_FROM_AA = 1.f / 8192.f;                         // 2^26 (A A)   -> 2^13 A A
+constexpr float X_FROM_XB = 1.f / 8192.f;                          // 2^25 (X B)   -> 2^12 X B
+constexpr int NORM_CHUNK = 8192;                                   // elements of one partial sum of squares
+
+struct Mat {
+    int rows, cols;          // as the caller holds it, contiguous
+    int Lp, Sp;              // padded
+    int y0, y1, a, b, slab, part;      // workspace offsets in units of 256 bytes
+};
+struct Io { const float *p, *g, *m; float *po, *mo; float k; };
+struct Mats { Mat m[CUTIE_MAX_BATCH]; int n; };
+struct Ios { Io io[CUTIE_MAX_BATCH]; };
+struct Starts { int v[CUTIE_MAX_BATCH + 1]; };      // first workgroup of each matrix
+struct Splits { short v[CUTIE_MAX_BATCH]; };
+struct Hyper {
+    float lr, mu, wd, l2, clip, grad_scale;
+    int nesterov;
+    const float* gnorm_sq;
+    const float* loss_scale;
+    const int32_t* invalid;
+};
+
+__device__ __forceinline__ int find(const Starts& s, int n, int id) {
+    int i = 0;
+    while (i + 1 < n && id >= s.v[i + 1]) ++i;
+    return i;
+}
+__device__ __forceinline__ char* at(char* ws, int off) { return ws + (int64_t)off * 256; }
+
+// the step is skipped: a gradient that is not finite, or results marked invalid
+__device__ __forceinline__ bool skip_step(const Hyper& h) {
+    return (h.invalid && *h.invalid != 0) || (h.gnorm_sq && !(fabsf(*h.gnorm_sq) <= 3.0e38f));
+}
+
+__device__ __forceinline__ void block_sum_f64(double v, double* out) {
+    __shared__ double sh[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) *out = ((sh[0] + sh[1]) + sh[2]) + sh[3];
+}
+
+// partial sums of squares of U, in f64 (squares of any f32 are in range), one per NORM_CHUNK elements.  MUON: U is made
+// here, m' stored, U left in the buffer that the first product overwrites later.
+template <bool MUON>
+__global__ __launch_bounds__(256) void ns_norm_kernel(Mats ms, Ios ios, Starts st, Hyper h, char* ws) {
+    const int i = find(st, ms.n, blockIdx.x), chunk = blockIdx.x - st.v[i];
+    const Mat M = ms.m[i];
+    const Io io = ios.io[i];
+    const int64_t n = (int64_t)M.rows * M.cols, e0 = (int64_t)chunk * NORM_CHUNK;
+    const int64_t e1 = min(n, e0 + NORM_CHUNK);
+    double s = 0;
+    if constexpr (!MUON) {
+        for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
+            const double v = io.g[e];
+            s = fma(v, v, s);
+        }
+    } else {
+        float* u = (float*)at(ws, M.y1);
+        const bool skip = skip_step(h);
+        const float inv = h.loss_scale ? h.loss_scale[1] : 1.f;
+        float scale = h.grad_scale;
+        if (h.gnorm_sq && h.clip > 0.f) scale *= h.clip / fmaxf(sqrtf(*h.gnorm_sq) * h.grad_scale, h.clip);
+        for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
+            const float g = (io.g[e] * inv + h.l2 * io.p[e]) * scale;
+            const float m0 = io.m[e];
+            const float m1 = h.mu * m0 + g;
+            const float v = h.nesterov ? g + h.mu * m1 : m1;
+            io.mo[e] = skip ? m0 : m1;
+            u[e] = v;
+            s = fma((double)v, (double)v, s);
+        }
+    }
+    block_sum_f64(s, (double*)at(ws, M.part) + chunk);
+}
+
+// v must exist as an f32 before it is narrowed.  Where it is a product the compiler may narrow straight out of the multiplier for
+// the stored hi (one rounding) and from the rounded f32 for the one that lo is taken against (two): next to a tie the pair is
+// then off by a whole step of f16 (one element of 8385 in the 65 x 129 test: 1.3e-5 in place of 3e-7).
+__device__ __forceinline__ void split(float v, f16_t& hi, f16_t& lo) {
+    asm volatile("" : "+v"(v));
+    hi = (f16_t)v;
+    lo = (f16_t)(v - (float)hi);
+}
+__device__ __forceinline__ void split4(const float* v, uint2& hi, uint2& lo) {
+    half4_t h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { f16_t a, b; split(v[e], a, b); h[e] = a; l[e] = b; }
+    hi = __builtin_bit_cast(uint2, h);
+    lo = __builtin_bit_cast(uint2, l);
+}
+__device__ __forceinline__ void join4(uint2 hi, uint2 lo, float* v) {
+    const half4_t h = __builtin_bit_cast(half4_t, hi), l = __builtin_bit_cast(half4_t, lo);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
+}
+// byte offset of value c (a multiple of 4) of a row's hi part; its lo part lies 64 bytes further
+__device__ __forceinline__ int64_t cell(int64_t row, int ld, int c) { return row * ((int64_t)ld * 4) + (c >> 5) * 128 + (c & 31) * 2; }
+
+// X0 in the work layout: a workgroup makes a 64 x 64 piece of [Lp][Sp]
+template <bool MUON>
+__global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts st, float eps, char* ws) {
+    __shared__ float tile[64][65];
+    __shared__ double total;
+    const int i = find(st, ms.n, blockIdx.x), id = blockIdx.x - st.v[i];
+    const Mat M = ms.m[i];
+    const float* src = MUON ? (const float*)at(ws, M.y1) : ios.io[i].g;
+    const int nt = M.Sp >> 6, l0 = (id / nt) << 6, s0 = (id % nt) << 6;
+    const bool flip = M.rows < M.cols;
+    // the norm: all partial sums, in one order
+    const int64_t parts = (((int64_t)M.rows * M.cols) + NORM_CHUNK - 1) / NORM_CHUNK;
+    const double* part = (const double*)at(ws, M.part);
+    double s = 0;
+    for (int64_t k = threadIdx.x; k < parts; k += 256) s += part[k];
+    block_sum_f64(s, &total);
+    const int c = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < 64; r += 4) {
+        // read along the caller's rows
+        const int row = (flip ? s0 : l0) + r, col = (flip ? l0 : s0) + c;
+        const float v = row < M.rows && col < M.cols ? src[(int64_t)row * M.cols + col] : 0.f;
+        if (flip) tile[c][r] = v;
+        else tile[r][c] = v;
+    }
+    __syncthreads();
+    const float k = (float)((double)X_SCALE / (sqrt(total) + (double)eps));
+    const int l = threadIdx.x >> 2, q = (threadIdx.x & 3) * 16;
+    char* out = at(ws, M.y0) + cell(l0 + l, M.Sp, s0 + q);
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+        float v[4];
+        uint2 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = tile[l][q + e + j] * k;
+        split4(v, hi, lo);
+        *reinterpret_cast<uint2*>(out + e * 2) = hi;
+        *reinterpret_cast<uint2*>(out + 64 + e * 2) = lo;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- products
+// Workgroup of 4 waves, 2 x 2, tile T x T with T = 32 F, a wave F x F fragments of 16 x 16.  A K step is 32 values: the tile's
+// 128-byte lines (hi and lo) go to LDS by buffer_load ... lds, two stages, the next one in flight while this one is used.
+template <int F> struct Shape {
+    static constexpr int T = 32 * F, HALF = T * 128, STAGE = 2 * HALF;      // bytes of one operand, of both
+    static constexpr int LDS = 2 * STAGE;
+    static constexpr int PIECES = T / 8;      // 1-KB pieces of an operand; a wave moves PIECES / 4 of each
+};
+__device__ __forceinline__ int tr_swz(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
+
+template <int F> struct Frags { short8_t hi[F], lo[F]; };
+
+template <int F>
+__device__ __forceinline__ void multiply(const Frags<F>& p, const Frags<F>& q, float4_t (&acc)[F][F]) {
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n) {
+            acc[m][n] = mma16<CUTIE_F16>(p.hi[m], q.hi[n], acc[m][n]);
+            acc[m][n] = mma16<CUTIE_F16>(p.hi[m], q.lo[n], acc[m][n]);
+            acc[m][n] = mma16<CUTIE_F16>(p.lo[m], q.hi[n], acc[m][n]);
+        }
+}
+
+// my pieces of the stage have landed and my reads of the other one are done; then everybody's are
+__device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// acc[m][n] += sum over K steps k0 .. k1 of P[p0 + m][k] * Q[q0 + n][k]: both operands row by row along K
+template <int F>
+__device__ __forceinline__ void product_rows(char* smem, const char* P, unsigned p_bytes, int p_rows, int p0, const char* Q, unsigned q_bytes,
+                                             int q_rows, int q0, int ld, int k0, int k1, float4_t (&acc)[F][F]) {
+    typedef Shape<F> S;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+    const u32x4s_t rp = make_rsrc(P, p_bytes), rq = make_rsrc(Q, q_bytes);
+    const unsigned lds0 = (unsigned)(uintptr_t)((lds_void_t*)smem);
+    unsigned po[S::PIECES / 4], qo[S::PIECES / 4];      // source offsets of this lane at K step 0
+#pragma unroll
+    for (int u = 0; u < S::PIECES / 4; ++u) {
+        const int row = (wave + 4 * u) * 8 + (lane >> 3);
+        const unsigned chunk = (unsigned)((lane & 7) ^ swz(row)) * 16u;
+        po[u] = p0 + row < p_rows ? (unsigned)(p0 + row) * (unsigned)(ld * 4) + chunk : BUF_OOB;
+        qo[u] = q0 + row < q_rows ? (unsigned)(q0 + row) * (unsigned)(ld * 4) + chunk : BUF_OOB;
+    }
+    auto issue = [&](int k, int buf) {
+        const unsigned d = (unsigned)k * 128u;
+#pragma unroll
+        for (int u = 0; u < S::PIECES / 4; ++u) {
+            const unsigned dst = lds0 + buf * S::STAGE + (wave + 4 * u) * 1024;
+            glds16(rp, dst, po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
+            glds16(rq, dst + S::HALF, qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
+        }
+    };
+    int pr[F], qr[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        const int m = (wm * F + f) * 16 + li, n = (wn * F + f) * 16 + li;
+        pr[f] = m * 128 + ((lg ^ swz(m)) << 4);
+        qr[f] = S::HALF + n * 128 + ((lg ^ swz(n)) << 4);
+    }
+    if (k0 < k1) issue(k0, 0);
+    for (int k = k0; k < k1; ++k) {
+        const int buf = (k - k0) & 1;
+        stage_ready();
+        if (k + 1 < k1) issue(k + 1, buf ^ 1);
+        const char* s = smem + buf * S::STAGE;
+        Frags<F> p, q;
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            p.hi[f] = *reinterpret_cast<const short8_t*>(s + pr[f]);
+            p.lo[f] = *reinterpret_cast<const short8_t*>(s + (pr[f] ^ 64));
+            q.hi[f] = *reinterpret_cast<const short8_t*>(s + qr[f]);
+            q.lo[f] = *reinterpret_cast<const short8_t*>(s + (qr[f] ^ 64));
+        }
+        multiply<F>(p, q, acc);
+    }
+}
+
+// acc[m][n] += sum over rows 32 k0 .. 32 k1 of X[r][p0 + m] * X[r][q0 + n]: K runs down the rows, so the fragments come through
+// the transposing LDS read.  A staged row holds T columns (hi and lo) = T * 4 bytes as 32-byte groups, XORed by the row.
+template <int F>
+__device__ __forceinline__ void product_cols(char* smem, const char* X, unsigned bytes, int cols, int p0, int q0, int k0, int k1,
+                                             float4_t (&acc)[F][F]) {
+    typedef Shape<F> S;
+    constexpr int ROWB = S::T * 4;                 // 512 or 256 bytes
+    constexpr int SLOTS = ROWB / 16;               // 16-byte slots of a staged row
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+    const u32x4s_t rs = make_rsrc(X, bytes);
+    const unsigned lds0 = (unsigned)(uintptr_t)((lds_void_t*)smem);
+    unsigned po[S::PIECES / 4], qo[S::PIECES / 4];
+#pragma unroll
+    for (int u = 0; u < S::PIECES / 4; ++u) {
+        const int slot = (wave + 4 * u) * 64 + lane, row = slot / SLOTS, w = slot % SLOTS;
+        const int byte = ((((w >> 1) ^ tr_swz(row)) << 1) | (w & 1)) * 16;      // of the row's T columns: 4 bytes a column
+        po[u] = p0 + byte / 4 < cols ? (unsigned)row * (unsigned)(cols * 4) + (unsigned)(p0 * 4 + byte) : BUF_OOB;
+        qo[u] = q0 + byte / 4 < cols ? (unsigned)row * (unsigned)(cols * 4) + (unsigned)(q0 * 4 + byte) : BUF_OOB;
+    }
+    auto issue = [&](int k, int buf) {
+        const unsigned d = (unsigned)k * 32u * (unsigned)(cols * 4);
+#pragma unroll
+        for (int u = 0; u < S::PIECES / 4; ++u) {
+            const unsigned dst = lds0 + buf * S::STAGE + (wave + 4 * u) * 1024;
+            glds16(rs, dst, po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
+            glds16(rs, dst + S::HALF, qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
+        }
+    };
+    const int r1 = lg * 8 + (li >> 2);      // and r1 + 4, whose swizzle is the same
+    unsigned pr[F], qr[F];
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+        const int m = wm * F + f, n = wn * F + f;      // 16-column fragments: 32-byte group (m >> 1) * 4 + plane * 2 + (m & 1)
+        pr[f] = lds0 + r1 * ROWB + ((((m >> 1) * 4 + (m & 1)) ^ tr_swz(r1)) * 32) + (li & 3) * 8;
+        qr[f] = lds0 + S::HALF + r1 * ROWB + ((((n >> 1) * 4 + (n & 1)) ^ tr_swz(r1)) * 32) + (li & 3) * 8;
+    }
+    auto tr2 = [&](unsigned a0) {
+        const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(a0));
+        const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(a0 + 4 * ROWB));
+        return short8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    };
+    if (k0 < k1) issue(k0, 0);
+    for (int k = k0; k < k1; ++k) {
+        const int buf = (k - k0) & 1;
+        stage_ready();
+        if (k + 1 < k1) issue(k + 1, buf ^ 1);
+        const unsigned o = buf * S::STAGE;
+        Frags<F> p, q;
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            p.hi[f] = tr2(pr[f] + o);
+            p.lo[f] = tr2((pr[f] ^ 64) + o);
+            q.hi[f] = tr2(qr[f] + o);
+            q.lo[f] = tr2((qr[f] ^ 64) + o);
+        }
+        multiply<F>(p, q, acc);
+    }
+}
+
+// lower-triangle tile `id` of a symmetric matrix: (row, col), col <= row
+__device__ __forceinline__ void tri(int id, int& r, int& c) {
+    r = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while (r * (r + 1) / 2 > id) --r;
+    while ((r + 1) * (r + 2) / 2 <= id) ++r;
+    c = id - r * (r + 1) / 2;
+}
+
+// The symmetric products A = X^T X (GRAM) and A A: the tiles on and below the diagonal, K cut into `splits` parts, f32
+// sums into slabs [split][tile][T][T].
+template <int F, bool GRAM>
+__global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats ms, Starts st, Splits sp, int which, char* ws) {
+    typedef Shape<F> S;
+    __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
+    const int i = find(st, ms.n, blockIdx.x);
+    const Mat M = ms.m[i];
+    const int nt = (M.Sp + S::T - 1) / S::T, tiles = nt * (nt + 1) / 2;
+    const int id = blockIdx.x - st.v[i], sl = id / tiles, t = id % tiles, splits = sp.v[i];
+    int r, c;
+    tri(t, r, c);
+    const int steps = (GRAM ? M.Lp : M.Sp) / 32, per = (steps + splits - 1) / splits;
+    const int k0 = min(steps, sl * per), k1 = min(steps, k0 + per);
+    float4_t acc[F][F];
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (GRAM) {
+        product_cols<F>(smem, at(ws, which ? M.y1 : M.y0), (unsigned)((int64_t)M.Lp * M.Sp * 4), M.Sp, r * S::T, c * S::T, k0, k1, acc);
+    } else {
+        const unsigned bytes = (unsigned)((int64_t)M.Sp * M.Sp * 4);
+        product_rows<F>(smem, at(ws, M.a), bytes, M.Sp, r * S::T, at(ws, M.a), bytes, M.Sp, c * S::T, M.Sp, k0, k1, acc);
+    }
+    // [n][m]: a lane holds four consecutive m of one n
+    float* out = (float*)at(ws, M.slab) + ((int64_t)sl * tiles + t) * (S::T * S::T);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n)
+            *reinterpret_cast<float4_t*>(out + ((wn * F + n) * 16 + li) * S::T + (wm * F + m) * 16 + lg * 4) = acc[m][n];
+}
+
+// slabs -> A (GRAM) or B = b A + c A A, both triangles: a workgroup folds a 32 x 32 piece of a tile in slab order
+template <int F, bool GRAM>
+__global__ __launch_bounds__(256) void ns_fold_kernel(Mats ms, Starts st, Splits sp, char* ws) {
+    typedef Shape<F> S;
+    __shared__ float tile[32][33];
+    const int i = find(st, ms.n, blockIdx.x);
+    const Mat M = ms.m[i];
+    const int nt = (M.Sp + S::T - 1) / S::T, tiles = nt * (nt + 1) / 2, splits = sp.v[i];
+    const int id = blockIdx.x - st.v[i], t = id / (F * F), piece = id % (F * F);
+    int r, c;
+    tri(t, r, c);
+    const int n = threadIdx.x >> 3, m = (threadIdx.x & 7) * 4;      // the piece's row and column
+    const int pn = (piece / F) * 32, pm = (piece % F) * 32;
+    const int gn = c * S::T + pn, gm = r * S::T + pm;               // of the whole matrix
+    if (gn >= M.Sp || gm >= M.Sp) return;
+    const float* src = (const float*)at(ws, M.slab) + (int64_t)t * (S::T * S::T) + (pn + n) * S::T + pm + m;
+    float4_t v = *reinterpret_cast<const float4_t*>(src);
+    for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const float4_t*>(src + (int64_t)k * tiles * (S::T * S::T));
+    float x[4];
+    uint2 hi, lo;
+    if constexpr (GRAM) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = v[e] * AB_FROM_XX;
+    } else {
+        const char* a = at(ws, M.a) + cell(gn + n, M.Sp, gm + m);
+        float old[4];
+        join4(*reinterpret_cast<const uint2*>(a), *reinterpret_cast<const uint2*>(a + 64), old);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(NS_B, old[e], NS_C * (v[e] * AB_FROM_AA));
+    }
+    char* dst = at(ws, GRAM ? M.a : M.b);
+    split4(x, hi, lo);
+    char* q = dst + cell(gn + n, M.Sp, gm + m);
+    *reinterpret_cast<uint2*>(q) = hi;
+    *reinterpret_cast<uint2*>(q + 64) = lo;
+    if (r == c) return;      // a diagonal tile holds both triangles itself
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[m + e][n] = x[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = tile[n][m + e];
+    split4(x, hi, lo);
+    q = dst + cell(gm + n, M.Sp, gn + m);
+    *reinterpret_cast<uint2*>(q) = hi;
+    *reinterpret_cast<uint2*>(q + 64) = lo;
+}
+
+// X' = a X + X B.  The last step (LAST) writes the caller's matrix: X itself, or (MUON) the parameters.
+template <int F, bool LAST, bool MUON>
+__global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Starts st, Hyper h, int which, char* ws) {
+    typedef Shape<F> S;
+    __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
+    const int i = find(st, ms.n, blockIdx.x);
+    const Mat M = ms.m[i];
+    const int nt = (M.Sp + S::T - 1) / S::T, id = blockIdx.x - st.v[i];
+    const int l0 = (id / nt) * S::T, s0 = (id % nt) * S::T;
+    const char* X = at(ws, which ? M.y1 : M.y0);
+    float4_t acc[F][F];
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
+    // rows of B (symmetric) against rows of X: a lane ends with four consecutive columns of one row of X
+    product_rows<F>(smem, at(ws, M.b), (unsigned)((int64_t)M.Sp * M.Sp * 4), M.Sp, s0, X, (unsigned)((int64_t)M.Lp * M.Sp * 4), M.Lp, l0,
+                    M.Sp, 0, M.Sp / 32, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+    const bool flip = M.rows < M.cols;
+    bool skip = false;
+    if constexpr (MUON) skip = skip_step(h);
+#pragma unroll
+    for (int n = 0; n < F; ++n) {
+        const int l = l0 + (wn * F + n) * 16 + li;
+        if (l >= M.Lp) continue;
+#pragma unroll
+        for (int m = 0; m < F; ++m) {
+            const int s = s0 + (wm * F + m) * 16 + lg * 4;
+            if (s >= M.Sp) continue;
+            const int64_t o = cell(l, M.Sp, s);
+            float x[4];
+            join4(*reinterpret_cast<const uint2*>(X + o), *reinterpret_cast<const uint2*>(X + o + 64), x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = fmaf(NS_A, x[e], acc[m][n][e] * X_FROM_XB);
+            if constexpr (!LAST) {
+                uint2 hi, lo;
+                split4(x, hi, lo);
+                char* q = at(ws, which ? M.y0 : M.y1) + o;
+                *reinterpret_cast<uint2*>(q) = hi;
+                *reinterpret_cast<uint2*>(q + 64) = lo;
+            } else {
+                const Io& io = ios.io[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = flip ? s + e : l, col = flip ? l : s + e;
+                    if (row >= M.rows || col >= M.cols) continue;
+                    const int64_t k = (int64_t)row * M.cols + col;
+                    const float v = x[e] * INV_X_SCALE;
+                    if constexpr (MUON) {
+                        const float p = io.p[k];
+                        io.po[k] = skip ? p : p * (1.f - h.lr * h.wd) - h.lr * io.k * v;
+                    } else {
+                        io.po[k] = v;
+                    }
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------- host
+struct NsPlan {
+    Mats ms;
+    Splits gram, square;
+    int fg, fs, fa;          // tile factors (4: 128 x 128, 2: 64 x 64) of the three products
+    size_t bytes;
+};
+
+inline int tri_tiles(int Sp, int f) { const int nt = (int)cdiv(Sp, 32 * f); return nt * (nt + 1) / 2; }
+
+// shapes: (rows, cols) of n matrices
+inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
+    CUTIE_CHECK_ARG(n >= 1 && n <= CUTIE_MAX_BATCH, "%s: %d matrices (1..%d)", who, n, CUTIE_MAX_BATCH);
+    p.ms.n = n;
+    for (int i = 0; i < n; ++i) {
+        const int r = shapes[2 * i], c = shapes[2 * i + 1];
+        CUTIE_CHECK_ARG(r >= 1 && c >= 1, "%s: matrix %d is %d x %d", who, i, r, c);
+        const int64_t Lp = cdiv(r > c ? r : c, 64) * 64, Sp = cdiv(r > c ? c : r, 64) * 64;
+        CUTIE_CHECK_ARG(Lp * Sp < ((int64_t)1 << 29), "%s: matrix %d is %d x %d (padded to multiples of 64, below 2^29 values)", who, i, r, c);
+        p.ms.m[i].rows = r;
+        p.ms.m[i].cols = c;
+        p.ms.m[i].Lp = (int)Lp;
+        p.ms.m[i].Sp = (int)Sp;
+    }
+    // the 128 tile where it alone gives the chip two workgroups a CU or (with K cut) K is long enough to be cut
+    int64_t tg = 0, ts = 0, ta = 0;
+    for (int i = 0; i < n; ++i) {
+        const Mat& m = p.ms.m[i];
+        tg += (int64_t)tri_tiles(m.Sp, 4) * cdiv(m.Lp, 256);
+        ts += (int64_t)tri_tiles(m.Sp, 4) * cdiv(m.Sp, 256);
+        ta += cdiv(m.Lp, 128) * cdiv(m.Sp, 128);
+    }
+    p.fg = tg >= 256 ? 4 : 2;
+    p.fs = ts >= 256 ? 4 : 2;
+    p.fa = ta >= 256 ? 4 : 2;
+    int64_t ng = 0, nq = 0;
+    for (int i = 0; i < n; ++i) { ng += tri_tiles(p.ms.m[i].Sp, p.fg); nq += tri_tiles(p.ms.m[i].Sp, p.fs); }
+    size_t off = 0;
+    auto take = [&](int64_t bytes) {
+        const size_t at = off;
+        off += (size_t)cdiv(bytes, 256);
+        return (int)at;
+    };
+    for (int i = 0; i < n; ++i) {
+        Mat& m = p.ms.m[i];
+        auto cut = [](int64_t want, int steps) {      // at least four K steps a part
+            int64_t s = want < steps / 4 ? want : steps / 4;
+            return (short)(s < 1 ? 1 : (s > 64 ? 64 : s));
+        };
+        p.gram.v[i] = cut(512 / ng, m.Lp / 32);
+        p.square.v[i] = cut(512 / nq, m.Sp / 32);
+        const int64_t y = (int64_t)m.Lp * m.Sp * 4, a = (int64_t)m.Sp * m.Sp * 4;
+        const int64_t sg = (int64_t)p.gram.v[i] * tri_tiles(m.Sp, p.fg) * (32 * p.fg) * (32 * p.fg) * 4;
+        const int64_t ss = (int64_t)p.square.v[i] * tri_tiles(m.Sp, p.fs) * (32 * p.fs) * (32 * p.fs) * 4;
+        m.y0 = take(y);
+        m.y1 = take(y);
+        m.a = take(a);
+        m.b = take(a);
+        m.slab = take(sg > ss ? sg : ss);
+        m.part = take(cdiv((int64_t)m.rows * m.cols, NORM_CHUNK) * 8);
+    }
+    CUTIE_CHECK_ARG(off < ((size_t)1 << 31), "%s: the matrices of one call are too large together", who);
+    p.bytes = off * 256;
+    return CUTIE_OK;
+}
+
+template <typename Count> inline unsigned starts(const NsPlan& p, Starts& st, Count count) {
+    int64_t t = 0;
+    for (int i = 0; i < p.ms.n; ++i) {
+        st.v[i] = (int)t;
+        t += count(p.ms.m[i], i);
+    }
+    st.v[p.ms.n] = (int)t;
+    return (unsigned)t;
+}
+
+template <int F, bool GRAM> inline void ns_sym(const NsPlan& p, int which, char* ws, hipStream_t stream) {
+    const Splits& sp = GRAM ? p.gram : p.square;
+    Starts st;
+    const unsigned g = starts(p, st, [&](const Mat& m, int i) { return (int64_t)tri_tiles(m.Sp, F) * sp.v[i]; });
+    hipLaunchKernelGGL((ns_sym_kernel<F, GRAM>), dim3(g), dim3(256), 0, stream, p.ms, st, sp, which, ws);
+    const unsigned f = starts(p, st, [&](const Mat& m, int) { return (int64_t)tri_tiles(m.Sp, F) * F * F; });
+    hipLaunchKernelGGL((ns_fold_kernel<F, GRAM>), dim3(f), dim3(256), 0, stream, p.ms, st, sp, ws);
+}
+
+template <int F, bool MUON>
+inline void ns_apply(const NsPlan& p, const Ios& ios, const Hyper& h, int which, bool last, char* ws, hipStream_t stream) {
+    Starts st;
+    const unsigned g = starts(p, st, [&](const Mat& m, int) { return cdiv(m.Lp, 32 * F) * cdiv(m.Sp, 32 * F); });
+    if (last) hipLaunchKernelGGL((ns_apply_kernel<F, true, MUON>), dim3(g), dim3(256), 0, stream, p.ms, ios, st, h, which, ws);
+    else hipLaunchKernelGGL((ns_apply_kernel<F, false, false>), dim3(g), dim3(256), 0, stream, p.ms, ios, st, h, which, ws);
+}
+
+template <bool MUON> inline int ns_run(const NsPlan& p, const Ios& ios, const Hyper& h, int steps, float eps, char* ws, hipStream_t stream) {
+    static_assert(sizeof(Mats) + sizeof(Ios) + sizeof(Starts) + sizeof(Hyper) + 64 < 4096, "kernel arguments");
+    Starts st;
+    const unsigned g0 = starts(p, st, [](const Mat& m, int) { return cdiv((int64_t)m.rows * m.cols, NORM_CHUNK); });
+    hipLaunchKernelGGL((ns_norm_kernel<MUON>), dim3(g0), dim3(256), 0, stream, p.ms, ios, st, h, ws);
+    CUTIE_CHECK_LAUNCH();
+    const unsigned g1 = starts(p, st, [](const Mat& m, int) { return (int64_t)(m.Lp / 64) * (m.Sp / 64); });
+    hipLaunchKernelGGL((ns_start_kernel<MUON>), dim3(g1), dim3(256), 0, stream, p.ms, ios, st, eps, ws);
+    CUTIE_CHECK_LAUNCH();
+    for (int k = 0; k < steps; ++k) {
+        const int which = k & 1;
+        if (p.fg == 4) ns_sym<4, true>(p, which, ws, stream);
+        else ns_sym<2, true>(p, which, ws, stream);
+        if (p.fs == 4) ns_sym<4, false>(p, which, ws, stream);
+        else ns_sym<2, false>(p, which, ws, stream);
+        if (p.fa == 4) ns_apply<4, MUON>(p, ios, h, which, k + 1 == steps, ws, stream);
+        else ns_apply<2, MUON>(p, ios, h, which, k + 1 == steps, ws, stream);
+        CUTIE_CHECK_LAUNCH();
+    }
+    return CUTIE_OK;
+}
+
+inline int ns_common(const char* who, int steps, float eps, const NsPlan& p, const void* ws, size_t bytes) {
+    CUTIE_CHECK_ARG(steps >= 1 && steps <= 32, "%s: steps=%d (1..32)", who, steps);
+    CUTIE_CHECK_ARG(eps > 0.f, "%s: eps=%g must be positive", who, (double)eps);
+    if (!ws || bytes < p.bytes || (reinterpret_cast<uintptr_t>(ws) & 255)) {
+        set_error("%s: workspace %zu < %zu (or not 256-byte aligned)", who, ws ? bytes : 0, p.bytes);
+        return CUTIE_E_WORKSPACE;
+    }
+    return CUTIE_OK;
+}
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+}  // namespace
+
+extern "C" size_t cutie_orthogonalize_workspace_bytes(const int* shapes, int n) {
+    NsPlan p;
+    if (!shapes || ns_plan("orthogonalize_workspace_bytes", shapes, n, p) != CUTIE_OK) return 0;
+    return p.bytes;
+}
+
+extern "C" int cutie_orthogonalize_batched(const cutie_orth_desc* descs, int n, int steps, float eps, void* workspace,
+                                           size_t workspace_bytes, cutie_stream_t stream_) {
+    CUTIE_CHECK_ARG(descs && n >= 1 && n <= CUTIE_MAX_BATCH, "orthogonalize: %d matrices (1..%d)", n, CUTIE_MAX_BATCH);
+    int shapes[2 * CUTIE_MAX_BATCH];
+    Ios ios = {};
+    for (int i = 0; i < n; ++i) {
+        shapes[2 * i] = descs[i].rows;
+        shapes[2 * i + 1] = descs[i].cols;
+        CUTIE_CHECK_ARG(descs[i].g && descs[i].out && aligned4(descs[i].g) && aligned4(descs[i].out),
+                        "orthogonalize: matrix %d: null or misaligned pointer", i);
+        ios.io[i].g = descs[i].g;
+        ios.io[i].po = descs[i].out;
+    }
+    NsPlan p;
+    if (int e = ns_plan("orthogonalize", shapes, n, p)) return e;
+    if (int e = ns_common("orthogonalize", steps, eps, p, workspace, workspace_bytes)) return e;
+    Hyper h = {};
+    return ns_run<false>(p, ios, h, steps, eps, (char*)workspace, (hipStream_t)stream_);
+}
+
+extern "C" int cutie_muon_step(const cutie_muon_desc* descs, int n, float lr, float momentum, int nesterov, float weight_decay, float l2,
+                               int steps, float eps, const float* gnorm_sq, float clip, float grad_scale, const float* loss_scale,
+                               const int32_t* invalid, void* workspace, size_t workspace_bytes, cutie_stream_t stream_) {
+    CUTIE_CHECK_ARG(descs && n >= 1 && n <= CUTIE_MAX_BATCH, "muon_step: %d matrices (1..%d)", n, CUTIE_MAX_BATCH);
+    CUTIE_CHECK_ARG(clip >= 0.f && (clip == 0.f || gnorm_sq), "muon_step: clip=%g needs gnorm_sq (0: no clip)", (double)clip);
+    int shapes[2 * CUTIE_MAX_BATCH];
+    Ios ios = {};
+    for (int i = 0; i < n; ++i) {
+        const cutie_muon_desc& d = descs[i];
+        shapes[2 * i] = d.rows;
+        shapes[2 * i + 1] = d.cols;
+        CUTIE_CHECK_ARG(d.p && d.g && d.m && d.p_out && d.m_out && aligned4(d.p) && aligned4(d.g) && aligned4(d.m) && aligned4(d.p_out) &&
+                            aligned4(d.m_out), "muon_step: matrix %d: null or misaligned pointer", i);
+        ios.io[i] = Io{d.p, d.g, d.m, d.p_out, d.m_out, d.out_scale};
+    }
+    NsPlan p;
+    if (int e = ns_plan("muon_step", shapes, n, p)) return e;
+    if (int e = ns_common("muon_step", steps, eps, p, workspace, workspace_bytes)) return e;
+    const Hyper h = {lr, momentum, weight_decay, l2, clip, grad_scale, nesterov, gnorm_sq, loss_scale, invalid};
+    return ns_run<true>(p, ios, h, steps, eps, (char*)workspace, (hipStream_t)stream_);
+}

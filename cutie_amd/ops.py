@@ -650,6 +650,98 @@ def opt_step(p, g, m, v, n_l2, wd, reg_scale, layers, dt, lr_t, beta1, beta2, ep
          ptr(extra_sq), ptr(loss_scale), ptr(invalid), ptr(gnorm_sq_out), ptr(reg_out), int(zero_from), stream(p.device))
 
 
+# ------------------------------------------------------------------------------------ K17
+ORTH_EPS = 1e-7
+
+
+def _matrix(t, what, like=None):
+    """a contiguous f32 tensor of at least two dimensions, as a [rows, cols] matrix: (rows, cols)"""
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() < 2:
+        raise capi.CutieError("%s: matrices must be contiguous f32 of at least two dimensions, got %s %s" % (what, t.dtype, tuple(t.shape)))
+    if like is not None and (t.shape != like.shape or t.device != like.device):
+        raise capi.CutieError("%s: tensors differ: %s on %s against %s on %s" % (what, tuple(t.shape), t.device, tuple(like.shape), like.device))
+    if t.numel() == 0:
+        raise capi.CutieError("%s: an empty matrix" % what)
+    return t.numel() // t.shape[-1], t.shape[-1]
+
+
+def _overlap(a, b):
+    return a.data_ptr() < b.data_ptr() + b.numel() * 4 and b.data_ptr() < a.data_ptr() + a.numel() * 4
+
+
+def orthogonalize_workspace_bytes(shapes):
+    """shapes: (rows, cols) of each matrix of one call, in order"""
+    flat = (ctypes.c_int * (2 * max(1, len(shapes))))(*[int(v) for s in shapes for v in s])
+    return capi.lib().cutie_orthogonalize_workspace_bytes(flat, len(shapes))
+
+
+def _orth_space(shapes, device, workspace, what):
+    if not 1 <= len(shapes) <= capi.MAX_BATCH:
+        raise capi.CutieError("%s: %d matrices (1..%d)" % (what, len(shapes), capi.MAX_BATCH))
+    need = orthogonalize_workspace_bytes(shapes)
+    if need == 0:
+        raise capi.CutieError("%s: %s" % (what, capi.lib().cutie_last_error().decode()))
+    return _workspace(workspace, need, device, what)
+
+
+def orthogonalize_batched(entries, steps=5, eps=ORTH_EPS, workspace=None):
+    """entries: list of (g, out), contiguous f32 of at least two dimensions taken as [rows, cols = last dimension] (a conv
+    kernel [kh,kw,cin,cout] as [kh*kw*cin, cout]); out = g with its singular values taken towards 1 by `steps` quintic
+    Newton-Schulz steps (cutie_orthogonalize_batched).  out may be g.  At most capi.MAX_BATCH matrices, one device."""
+    arr = (capi.OrthDesc * max(1, len(entries)))()
+    shapes = []
+    for i, (g, out) in enumerate(entries[:capi.MAX_BATCH]):
+        shapes.append(_matrix(g, "orthogonalize"))
+        _matrix(out, "orthogonalize", g)
+        if g.device != entries[0][0].device:
+            raise capi.CutieError("orthogonalize: matrices on different devices")
+        arr[i].g, arr[i].out, arr[i].rows, arr[i].cols = ptr(g), ptr(out), shapes[-1][0], shapes[-1][1]
+    ws = _orth_space(shapes if len(entries) <= capi.MAX_BATCH else entries, entries[0][0].device if entries else None, workspace,
+                     "orthogonalize")
+    call("cutie_orthogonalize_batched", arr, len(entries), int(steps), float(eps), ptr(ws), ws.numel() * ws.element_size(),
+         stream(ws.device))
+
+
+def muon_descs(entries):
+    """entries: list of (p, g, m, p_out, m_out, out_scale), contiguous f32 matrices as orthogonalize_batched takes them; p_out
+    may be p and m_out may be m (an update in place) -> what muon_step and replays of it take: (host descriptor array, shapes,
+    device).  The tensors must outlive it."""
+    if not 1 <= len(entries) <= capi.MAX_BATCH:
+        raise capi.CutieError("muon_step: %d matrices (1..%d)" % (len(entries), capi.MAX_BATCH))
+    arr = (capi.MuonDesc * len(entries))()
+    shapes = []
+    for i, (p, g, m, p_out, m_out, out_scale) in enumerate(entries):
+        shapes.append(_matrix(p, "muon_step"))
+        for t in (g, m, p_out, m_out):
+            _matrix(t, "muon_step", p)
+        if p.device != entries[0][0].device:
+            raise capi.CutieError("muon_step: matrices on different devices")
+        if any(_overlap(a, b) for a, b in ((p_out, g), (p_out, m), (p_out, m_out), (m_out, g), (m_out, p))):
+            raise capi.CutieError("muon_step: matrix %d: an output overlaps another tensor" % i)
+        if any(_overlap(a, b) and a.data_ptr() != b.data_ptr() for a, b in ((p_out, p), (m_out, m))):
+            raise capi.CutieError("muon_step: matrix %d: an output may be its input, not overlap a part of it" % i)
+        d = arr[i]
+        d.p, d.g, d.m, d.p_out, d.m_out = ptr(p), ptr(g), ptr(m), ptr(p_out), ptr(m_out)
+        d.rows, d.cols, d.out_scale = shapes[-1][0], shapes[-1][1], float(out_scale)
+    return arr, shapes, entries[0][0].device
+
+
+def muon_step(entries, lr, momentum=0.95, nesterov=True, weight_decay=0.0, l2=0.0, steps=5, eps=ORTH_EPS, gnorm_sq=None, clip=0.0,
+              grad_scale=1.0, loss_scale=None, invalid=None, workspace=None):
+    """One orthogonalised update of up to capi.MAX_BATCH matrices (cutie_muon_step): entries as muon_descs takes them, or what it
+    returned.  gnorm_sq: f32 [1] squared global norm on the device, for the clip and to skip a step that is not finite;
+    loss_scale: the K12 state; invalid: int32 [1], non-zero skips the step.  workspace: optional uint8 tensor of
+    orthogonalize_workspace_bytes(shapes) bytes."""
+    arr, shapes, device = entries if isinstance(entries, tuple) else muon_descs(entries)
+    ws = _orth_space(shapes, device, workspace, "muon_step")
+    for t, what, dt in ((gnorm_sq, "gnorm_sq", torch.float32), (loss_scale, "loss_scale", torch.float32), (invalid, "invalid", torch.int32)):
+        if t is not None and (t.dtype != dt or t.device != device):
+            raise capi.CutieError("muon_step: %s must be %s on %s" % (what, dt, device))
+    call("cutie_muon_step", arr, len(arr), float(lr), float(momentum), 1 if nesterov else 0, float(weight_decay), float(l2), int(steps),
+         float(eps), ptr(gnorm_sq), float(clip), float(grad_scale), ptr(loss_scale), ptr(invalid), ptr(ws),
+         ws.numel() * ws.element_size(), stream(device))
+
+
 def batch_scatter_add(dout, idx, dfeat):
     """dout [B, n_cells, >=C] view; idx int32 [B, n_cells]; dfeat f32 [B, n_src, C] contiguous, caller-zeroed."""
     B, n_src, C = dfeat.shape

@@ -538,6 +538,46 @@ int cutie_opt_step(float* p, float* g, float* m, float* v, int64_t n, int64_t n_
                    float* loss_scale /* nullable */, const int32_t* invalid /* nullable */,
                    float* gnorm_sq_out, float* reg_out, int64_t zero_from, cutie_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * K17  orthogonalised update: an optimizer step for matrices (the conv kernels as [kh*kw*cin][cout]) beside K12's Adam.   No
+ *     counterpart in the reference, which has Adam only (main_train_json.py:153).
+ * orthogonalize:  X = g / (|g|_F + eps), then `steps` times X <- a X + X (b A + c A A), A = X^T X (X X^T of a wide matrix: the
+ *     same map), a = 3.4445, b = -4.7750, c = 2.0315;  out = X, f32.  out may be g.  steps = 1 .. 32, eps > 0.
+ * muon_step:  g' = (g / S + l2 * p) * grad_scale * (clip > 0 ? clip / max(sqrt(*gnorm_sq) * grad_scale, clip) : 1)
+ *     m_out = momentum * m + g';   u = nesterov ? g' + momentum * m_out : m_out
+ *     p_out = p * (1 - lr * weight_decay) - lr * out_scale * orthogonalize(u)
+ *     p_out may be p, m_out may be m; nothing else may overlap.  S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq
+ *     (nullable; the squared norm with S taken out, as cutie_opt_step leaves it) that is not finite or *invalid != 0 (nullable)
+ *     makes p_out = p, m_out = m.
+ * The products run on the matrix cores at f32 accuracy: operands are two f16 (22 bits), sums f32, sums of squares f64, all in
+ * a fixed order: the same bits every run for one list of shapes.  X is kept to 2^-36: of a matrix whose norm is below eps, so
+ * much less of the (small) result is left.
+ * Matrices are contiguous f32 [rows][cols], any size from 1 x 1 to 2^29 values (padded to multiples of 64), up to
+ * CUTIE_MAX_BATCH a call, in one set of launches.  descs / shapes (rows, cols of each matrix) are HOST arrays.
+ * workspace: cutie_orthogonalize_workspace_bytes(shapes, n) bytes for the same shapes in the same order, 256-byte aligned,
+ * clobbered, no pre-fill (0 for shapes that the call would refuse). */
+typedef struct cutie_orth_desc {
+    const float* g;
+    float* out;
+    int rows, cols;
+} cutie_orth_desc;
+typedef struct cutie_muon_desc {
+    const float* p;
+    const float* g;
+    const float* m;
+    float* p_out;
+    float* m_out;
+    int rows, cols;
+    float out_scale;
+} cutie_muon_desc;
+size_t cutie_orthogonalize_workspace_bytes(const int* shapes /* host [n][2] */, int n);
+int cutie_orthogonalize_batched(const cutie_orth_desc* descs /* host */, int n, int steps, float eps,
+                                void* workspace, size_t workspace_bytes, cutie_stream_t stream);
+int cutie_muon_step(const cutie_muon_desc* descs /* host */, int n, float lr, float momentum, int nesterov,
+                    float weight_decay, float l2, int steps, float eps, const float* gnorm_sq /* nullable */, float clip,
+                    float grad_scale, const float* loss_scale /* nullable */, const int32_t* invalid /* nullable */,
+                    void* workspace, size_t workspace_bytes, cutie_stream_t stream);
+
 /* K13  Model.positional_sampling, model_framework.py:73-86 (tf.batch_gather):
  * out[b, cell, :] = feat[b, idx[b, cell], :].  An index outside [0, n_src) is clamped into it and bumps *oob_count
  * (int32, nullable, caller-zeroed): tf.batch_gather raises on such an index, the caller raises from the counter. */
