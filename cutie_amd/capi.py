@@ -171,9 +171,11 @@ def stream(device=None):
     trailing stream()), not of whatever device happens to be current on the calling thread.  `device` overrides, for
     calls whose pointers sit inside a descriptor array."""
     if device is not None:
-        _tls.dev = torch.device(device)
+        _tls.dev = device if isinstance(device, torch.device) else torch.device(device)
     dev = getattr(_tls, "dev", None)
-    return torch.cuda.current_stream(dev).cuda_stream
+    if dev is None or dev.index is None:
+        return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)      # the same handle without a Stream object (0.1 against 2 us)
 
 
 def dt_of(t):
@@ -214,13 +216,13 @@ def ptr(t):
 def ld_of(t):
     """leading dimension (elements) of a [..., C] view whose rows are dense in the last axis
     and whose leading axes collapse to one row index"""
-    if t.stride(-1) != 1:
+    strides, shape = t.stride(), t.shape
+    if strides[-1] != 1:
         raise CutieError("channel axis must be contiguous")
-    ld = t.stride(-2)
-    for d in range(t.dim() - 2):
-        if t.stride(d) != t.stride(d + 1) * t.shape[d + 1]:
-            raise CutieError("view is not row-collapsible: shape %s strides %s" % (tuple(t.shape), t.stride()))
-    return ld
+    for d in range(len(strides) - 2):
+        if strides[d] != strides[d + 1] * shape[d + 1]:
+            raise CutieError("view is not row-collapsible: shape %s strides %s" % (tuple(shape), strides))
+    return strides[-2]
 
 
 def call(name, *args):

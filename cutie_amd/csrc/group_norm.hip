@@ -7,9 +7,16 @@
 //   dx = rstd * (h - sum h / N - xhat * sum (h * xhat) / N)
 // Both directions are HBM-bound: 2 (forward) or 3 (backward) tensors moved, ~12 / ~25 operations an element.
 //
-// Two forms.  RESIDENT: a workgroup owns whole groups of one sample and keeps their values in registers between the sums
-// and the store, so each tensor is moved once.  SPLIT, where a group does not fit a workgroup: per-channel sums over
+// Two forms.  RESIDENT: a workgroup owns whole groups of one sample and keeps their values in registers (and LDS) between the
+// sums and the store, so each tensor is moved once.  SPLIT, where a group does not fit a workgroup: per-channel sums over
 // slices of HW, a small fold, and a second pass over the operands.
+//
+// Measured, 32 x 64 x 64 x 256, 32 groups (134 MB forward, 201 MB backward), MI355X: forward f16 30 us resident (4.4 TB/s; split
+// 52), backward bf16 SiLU 54 us + 5 us fold (3.7 TB/s; split 95).  What decides is the width of the piece of a pixel that a
+// workgroup reads (its groups' channels): 16 bytes 50 us forward, 32 bytes 31, 64 bytes 30 - L2 hands out 64 bytes at least -
+// and, backward, one exponential and one reciprocal an element instead of two (86 us when the store pass made g again).
+// Non-temporal stores: 38 and 90 us (pieces of a line no longer meet in L2).  One document (B = 1): 12 us on 32 CUs, the latency of
+// a load, two sums and 4 us of arithmetic.
 #include "common.h"
 
 namespace {
@@ -35,37 +42,49 @@ template <int DT> struct Pack<DT, 1> {
     __device__ __forceinline__ void store(T* p) const { *p = v; }
 };
 
-// 1 / (1 + exp(-z)).  f32: the library's expf and divide.  16-bit outputs take the hardware exponential and reciprocal
-// (a few units of 2^-23): half a step of the output is 2^-11 (f16) or 2^-8 (bf16).
+// The loops are written once per activation (with_act): the choice is uniform, and left inside a loop it costs a third of the
+// instructions of a kernel whose arithmetic is as long as its memory traffic.
+template <int A> struct Act { static constexpr int v = A; };
+template <typename F> __device__ __forceinline__ void with_act(int act, F&& f) {
+    switch (act) {
+        case GN_ACT_RELU: f(Act<GN_ACT_RELU>()); break;
+        case GN_ACT_SIGMOID: f(Act<GN_ACT_SIGMOID>()); break;
+        case GN_ACT_SILU: f(Act<GN_ACT_SILU>()); break;
+        default: f(Act<GN_ACT_NONE>());
+    }
+}
+
+// 1 / (1 + exp(-z)).  f32: the library's expf and divide.  16-bit outputs take the hardware exponential and reciprocal (a few units of 2^-23): half a
+// step of the output is 2^-11 (f16) or 2^-8 (bf16).
 template <int DT> __device__ __forceinline__ float sigmoid_of(float z) {
     if constexpr (DT == CUTIE_F32) return 1.f / (1.f + expf(-z));
-    else return __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
-template <int DT> __device__ __forceinline__ float act_of(float z, int act) {
-    if (act == GN_ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays NaN
-    if (act == GN_ACT_SIGMOID) return sigmoid_of<DT>(z);
-    if (act == GN_ACT_SILU) return z * sigmoid_of<DT>(z);
+template <int DT, int A> __device__ __forceinline__ float act_of(float z) {
+    if constexpr (A == GN_ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays NaN
+    if constexpr (A == GN_ACT_SIGMOID) return sigmoid_of<DT>(z);
+    if constexpr (A == GN_ACT_SILU) return z * sigmoid_of<DT>(z);
     return z;
 }
 
 // act'(z) at z = gamma * xhat + beta.  The step of the ReLU is the one place where a rounding error of z is not a small
 // error of the gradient: where |z| is within the f32 error of its own computation (d = x - mean, a product and a sum: at
 // most 3 roundings, 2^-24 each, of |d * rg| + |beta|; 4e-7 > 3 * 2^-24) the sign is taken in f64.
-template <int DT>
-__device__ __forceinline__ float act_grad(float x, float mean, float rstd, float gamma, float beta, int act) {
-    if (act == GN_ACT_NONE) return 1.f;
-    const float d = x - mean, rg = rstd * gamma;
-    const float z = fmaf(d, rg, beta);
-    if (act == GN_ACT_RELU) {
-        if (fabsf(z) <= 4e-7f * (fabsf(d * rg) + fabsf(beta))) {
-            const double z64 = ((double)x - (double)mean) * (double)rstd * (double)gamma + (double)beta;
+// gamma: the channel's, nullable (1).
+struct Norm1 { float mean, rstd, beta, rg; };      // of one channel; rg = rstd * gamma
+template <int DT, int A> __device__ __forceinline__ float act_grad(float x, float d, const Norm1& n, const float* gamma) {
+    if constexpr (A == GN_ACT_NONE) return 1.f;
+    const float z = fmaf(d, n.rg, n.beta);
+    if constexpr (A == GN_ACT_RELU) {
+        if (__builtin_expect(fabsf(z) <= 4e-7f * (fabsf(d * n.rg) + fabsf(n.beta)), 0)) {
+            const double z64 = ((double)x - (double)n.mean) * (double)n.rstd * (gamma ? (double)*gamma : 1.0) + (double)n.beta;
             return z64 > 0.0 ? 1.f : 0.f;
         }
         return z > 0.f ? 1.f : (z != z ? z : 0.f);
     }
-    const float s = sigmoid_of<DT>(z);
-    if (act == GN_ACT_SIGMOID) return s * (1.f - s);
-    return s * (1.f + z * (1.f - s));
+    const float s = sigmoid_of<DT>(z), r = 1.f - s;
+    if constexpr (A == GN_ACT_SIGMOID) return s * r;
+    return s * fmaf(z, r, 1.f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- resident
@@ -75,6 +94,7 @@ struct GnShape {
     int cv;             // vectors per pixel of a workgroup: gc * Cg / VEC
     int rows_par;       // pixels side by side: blockDim / cv
     int64_t items;      // B * G / gc
+    bool fast;          // cv and cv / gc are powers of two up to 64: sums by lane exchanges
 };
 
 // Workgroups that share 128-byte lines (the groups of one pixel) go to one XCD: dispatch deals consecutive blocks to the
@@ -84,25 +104,111 @@ __device__ __forceinline__ int64_t xcd_item(int64_t items) {
     return (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
 }
 
-// sum over the threads of each group: every thread leaves its value, wave w folds groups w, w + waves, ... in a fixed
-// order, every thread takes its group's.  thread t's group is (t % cv) / (cv / gc).
-__device__ __forceinline__ float group_sum(float v, float* sh, float* tot, int gc, int cv, int active, int my) {
-    __syncthreads();
-    sh[threadIdx.x] = v;
-    __syncthreads();
+// Sums of NV values over the threads of each group; thread t's group is (t % cv) / vpg, vpg = cv / gc vectors a pixel.
+// Where cv and vpg are powers of two up to 64 (`fast`) the lanes of one group meet by exchanges, then the waves in LDS in wave
+// order; else every thread leaves its value and wave w folds groups w, w + waves, ... in a fixed order.
+// sh: 16 * 64 * NV floats (1024 * NV).  The caller synchronises before it uses sh again.
+template <int NV>
+__device__ __forceinline__ void group_sums(float (&v)[NV], float* sh, const GnShape& s, int my) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int vpg = cv / gc, n = active / gc;       // vectors of a group in a pixel; threads of a group
-    for (int g = wave; g < gc; g += waves) {
-        float s = 0.f;
-        for (int i = lane; i < n; i += 64) {
-            const int r = i / vpg;
-            s += sh[r * cv + g * vpg + (i - r * vpg)];
+    const int vpg = s.cv / s.gc;
+    if (s.fast) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+            if (o >= s.cv || o < vpg) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) v[k] += __shfl_xor(v[k], o, 64);
+            }
+        if (lane < s.cv && (lane & (vpg - 1)) == 0) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) sh[(my * NV + k) * 16 + wave] = v[k];
         }
-        s = wave_sum(s);
-        if (lane == 0) tot[g] = s;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const float* q = sh + (my * NV + k) * 16;
+            float t = 0.f;
+            for (int w = 0; w < waves; ++w) t += q[w];
+            v[k] = t;
+        }
+        return;
+    }
+    __shared__ float tot[NV][1024];
+    const int active = s.rows_par * s.cv, n = active / s.gc;       // threads that hold values; of them in one group
+#pragma unroll
+    for (int k = 0; k < NV; ++k) sh[k * 1024 + threadIdx.x] = v[k];
+    __syncthreads();
+    for (int g = wave; g < s.gc; g += waves) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float t = 0.f;
+            for (int i = lane; i < n; i += 64) {
+                const int r = i / vpg;
+                t += sh[k * 1024 + r * s.cv + g * vpg + (i - r * vpg)];
+            }
+            t = wave_sum(t);
+            if (lane == 0) tot[k][g] = t;
+        }
     }
     __syncthreads();
-    return tot[my];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] = tot[k][my];
+}
+
+// chan[c][2] = (sum of sx, sum of sg) of each channel of the workgroup over its pixels.  fast: the pixels of a wave meet by
+// exchanges that halve the values a lane holds (8 + 4 + 2 + 1 of them for 16 values), then the waves in LDS in wave order.
+template <int VEC>
+__device__ __forceinline__ void channel_sums(const float* sx, const float* sg, float* part, const GnShape& s, float* chan) {
+    constexpr int NV = 2 * VEC;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int n = s.cv * VEC;
+    if (s.fast) {
+        float v[NV];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { v[e] = sx[e]; v[VEC + e] = sg[e]; }
+        int base = 0, left = NV;
+#pragma unroll
+        for (int st = 0; st < 6; ++st) {
+            const int o = 32 >> st, half = (NV >> st) / 2;      // half: compile-time
+            if (o < s.cv) break;
+            if (half >= 1) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int i = 0; i < half; ++i) {
+                    const float keep = up ? v[i + half] : v[i], send = up ? v[i] : v[i + half];
+                    v[i] = keep + __shfl_xor(send, o, 64);
+                }
+                base += up ? half : 0;
+                left = half;
+            } else {
+                v[0] += __shfl_xor(v[0], o, 64);
+            }
+        }
+        float* q = part + (wave * NV + base) * s.cv + (lane & (s.cv - 1));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < left) q[i * s.cv] = v[i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < NV * s.cv; i += blockDim.x) {
+            float t = 0.f;
+            for (int w = 0; w < waves; ++w) t += part[w * NV * s.cv + i];
+            const int k = i / s.cv, c = (i - k * s.cv) * VEC + (k & (VEC - 1));
+            chan[c * 2 + (k >= VEC ? 1 : 0)] = t;
+        }
+        return;
+    }
+    float* p0 = part + threadIdx.x * VEC;
+    float* p1 = p0 + blockDim.x * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { p0[e] = sx[e]; p1[e] = sg[e]; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
+        const int k = i / n, c = i - k * n;
+        const float* q = part + k * blockDim.x * VEC + c;
+        float t = 0.f;
+        for (int r = 0; r < s.rows_par; ++r) t += q[r * n];
+        chan[c * 2 + k] = t;
+    }
 }
 
 template <int DT, int VEC, int K>
@@ -110,15 +216,14 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(const typename elem<DT>:
                                                         const float* __restrict__ gamma, const float* __restrict__ beta, float eps,
                                                         int act, typename elem<DT>::type* __restrict__ y, int ld_y,
                                                         float* __restrict__ stats, GnShape s) {
-    __shared__ float sh[1024];
-    __shared__ float tot[1024];
+    __shared__ float sh1[1024];
+    __shared__ float sh2[2 * 1024];
     const int64_t item = xcd_item(s.items);
     if (item >= s.items) return;
     const int per = s.G / s.gc;
     const int64_t b = item / per;
     const int g0 = (int)(item - b * per) * s.gc;
-    const int active = s.rows_par * s.cv;
-    const bool on = (int)threadIdx.x < active;
+    const bool on = (int)threadIdx.x < s.rows_par * s.cv;
     const int col = threadIdx.x % s.cv, row = threadIdx.x / s.cv;
     const int my = on ? col / (s.cv / s.gc) : 0;
     const int c0 = g0 * s.Cg + col * VEC;
@@ -130,24 +235,25 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(const typename elem<DT>:
         if (on && r < s.HW) d[k].load(px + (int64_t)r * ld_x);
     }
     const float inv_n = 1.f / ((float)s.HW * (float)s.Cg);
-    float a = 0.f;
+    float sum[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (on && row + k * s.rows_par < s.HW) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a += d[k].get(e);
+            for (int e = 0; e < VEC; ++e) sum[0] += d[k].get(e);
         }
-    const float mean0 = group_sum(a, sh, tot, s.gc, s.cv, active, my) * inv_n;
+    group_sums<1>(sum, sh1, s, my);
+    const float mean0 = sum[0] * inv_n;
     // second moments about mean0, and what mean0 misses of the mean (its own rounding): d1
-    float q1 = 0.f, q2 = 0.f;
+    float q[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (on && row + k * s.rows_par < s.HW) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) { const float t = d[k].get(e) - mean0; q1 += t; q2 = fmaf(t, t, q2); }
+            for (int e = 0; e < VEC; ++e) { const float t = d[k].get(e) - mean0; q[0] += t; q[1] = fmaf(t, t, q[1]); }
         }
-    const float d1 = group_sum(q1, sh, tot, s.gc, s.cv, active, my) * inv_n;
-    const float m2 = group_sum(q2, sh, tot, s.gc, s.cv, active, my) * inv_n;
+    group_sums<2>(q, sh2, s, my);
+    const float d1 = q[0] * inv_n, m2 = q[1] * inv_n;
     const float var = fmaxf(m2 - d1 * d1, 0.f) + (m2 - m2);      // + (m2 - m2): fmaxf drops a NaN, the group must keep it
     const float rstd = 1.f / sqrtf(var + eps);
     if (!on) return;
@@ -163,103 +269,119 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(const typename elem<DT>:
         be[e] = fmaf(-d1, rg[e], beta ? beta[c0 + e] : 0.f);
     }
     typename elem<DT>::type* py = y + (b * s.HW) * ld_y + c0;
+    with_act(act, [&](auto A) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int r = row + k * s.rows_par;
-        if (r < s.HW) {
+        for (int k = 0; k < K; ++k) {
+            const int r = row + k * s.rows_par;
+            if (r < s.HW) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) d[k].set(e, act_of<DT>(fmaf(d[k].get(e) - mean0, rg[e], be[e]), act));
-            d[k].store(py + (int64_t)r * ld_y);
+                for (int e = 0; e < VEC; ++e) d[k].set(e, act_of<DT, decltype(A)::v>(fmaf(d[k].get(e) - mean0, rg[e], be[e])));
+                d[k].store(py + (int64_t)r * ld_y);
+            }
         }
-    }
+    });
 }
 
-// chan (nullable) f32 [B][C][2]: (sum g * xhat, sum g) of each sample and channel, folded over b by gn_fold_params
+// chan (nullable) f32 [B][C][2]: (sum g * xhat, sum g) of each sample and channel, folded over b by gn_fold_params.
+// dy and x are read once, four vectors ahead of their use; g = dy act'(z) stays in registers as f32 (its exponential and
+// reciprocal are 32 of the 88 cycles that an element takes up to the sums), x as it came in LDS (vectors) or registers.
 template <int DT, int VEC, int K>
-__global__ __launch_bounds__(1024) void gn_bwd_resident(const typename elem<DT>::type* __restrict__ dy, int ld_dy,
-                                                        const typename elem<DT>::type* __restrict__ x, int ld_x,
-                                                        const float* __restrict__ gamma, const float* __restrict__ beta, int act,
-                                                        const float* __restrict__ stats, typename elem<DT>::type* __restrict__ dx,
-                                                        int ld_dx, float* __restrict__ chan, GnShape s) {
-    extern __shared__ float part[];         // [2][blockDim][VEC] when chan is wanted
-    __shared__ float sh[1024];
-    __shared__ float tot[1024];
+__global__ __launch_bounds__(VEC > 1 ? 512 : 1024) void gn_bwd_resident(const typename elem<DT>::type* __restrict__ dy, int ld_dy,
+                                                                        const typename elem<DT>::type* __restrict__ x, int ld_x,
+                                                                        const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                                        int act, const float* __restrict__ stats,
+                                                                        typename elem<DT>::type* __restrict__ dx, int ld_dx,
+                                                                        float* __restrict__ chan, GnShape s) {
+    typedef Pack<DT, VEC> P;
+    constexpr bool XL = VEC > 1;
+    extern __shared__ __attribute__((aligned(16))) char dyn[];      // x [K][blockDim] vectors (XL); later the channel sums
+    __shared__ float sh[2 * 1024];
     const int64_t item = xcd_item(s.items);
     if (item >= s.items) return;
     const int per = s.G / s.gc;
     const int64_t b = item / per;
     const int g0 = (int)(item - b * per) * s.gc;
-    const int active = s.rows_par * s.cv;
-    const bool on = (int)threadIdx.x < active;
+    const bool on = (int)threadIdx.x < s.rows_par * s.cv;
     const int col = threadIdx.x % s.cv, row = threadIdx.x / s.cv;
     const int my = on ? col / (s.cv / s.gc) : 0;
     const int c0 = g0 * s.Cg + col * VEC;
-    Pack<DT, VEC> vx[K], vd[K];
     const typename elem<DT>::type* px = x + (b * s.HW) * ld_x + c0;
     const typename elem<DT>::type* pd = dy + (b * s.HW) * ld_dy + c0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int r = row + k * s.rows_par;
-        if (on && r < s.HW) {
-            vx[k].load(px + (int64_t)r * ld_x);
-            vd[k].load(pd + (int64_t)r * ld_dy);
-        }
-    }
+    P* keep = reinterpret_cast<P*>(dyn) + threadIdx.x;
+    P kx[XL ? 1 : K];
     const float mean = stats[(b * s.G + g0 + my) * 2], rstd = stats[(b * s.G + g0 + my) * 2 + 1];
-    float ga[VEC], be[VEC], sg[VEC], sx[VEC];
+    Norm1 ch[VEC];
+    float sg[VEC], sx[VEC];      // sums of g and g * (x - mean)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        ga[e] = on && gamma ? gamma[c0 + e] : 1.f;
-        be[e] = on && beta ? beta[c0 + e] : 0.f;
+        ch[e].mean = mean;
+        ch[e].rstd = rstd;
+        ch[e].beta = on && beta ? beta[c0 + e] : 0.f;
+        ch[e].rg = on && gamma ? rstd * gamma[c0 + e] : rstd;
         sg[e] = 0.f;
         sx[e] = 0.f;
     }
+    with_act(act, [&](auto A) {
+        float g[K][VEC];
+        constexpr int AHEAD = K < 4 ? K : 4;
+        P vx[AHEAD], vd[AHEAD];
+        auto fetch = [&](int k) {
+            const int r = row + k * s.rows_par;
+            if (on && r < s.HW) {
+                vx[k % AHEAD].load(px + (int64_t)r * ld_x);
+                vd[k % AHEAD].load(pd + (int64_t)r * ld_dy);
+            }
+        };
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-        if (on && row + k * s.rows_par < s.HW) {
+        for (int k = 0; k < AHEAD; ++k) fetch(k);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const bool in = on && row + k * s.rows_par < s.HW;
+            const P cx = vx[k % AHEAD], cd = vd[k % AHEAD];
+            if (k + AHEAD < K) fetch(k + AHEAD);
+            if constexpr (XL) keep[k * blockDim.x] = cx;
+            else kx[k] = cx;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float xe = vx[k].get(e);
-                const float g = vd[k].get(e) * act_grad<DT>(xe, mean, rstd, ga[e], be[e], act);
-                sg[e] += g;
-                sx[e] = fmaf(g, (xe - mean) * rstd, sx[e]);
+                g[k][e] = 0.f;
+                if (in) {
+                    const float xe = cx.get(e), d = xe - mean;
+                    g[k][e] = cd.get(e) * act_grad<DT, decltype(A)::v>(xe, d, ch[e], gamma ? gamma + c0 + e : nullptr);
+                    sg[e] += g[k][e];
+                    sx[e] = fmaf(g[k][e], d, sx[e]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);      // one vector at a time: unrolled freely, the registers do not hold it
         }
-    float h0 = 0.f, h1 = 0.f;
+        float h[2] = {0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) { h0 = fmaf(sg[e], ga[e], h0); h1 = fmaf(sx[e], ga[e], h1); }
-    const float inv_n = 1.f / ((float)s.HW * (float)s.Cg);
-    const float s0 = group_sum(h0, sh, tot, s.gc, s.cv, active, my) * inv_n;
-    const float s1 = group_sum(h1, sh, tot, s.gc, s.cv, active, my) * inv_n;
+        for (int e = 0; e < VEC; ++e) {
+            h[0] = fmaf(sg[e], ch[e].rg, h[0]);
+            h[1] = fmaf(sx[e], ch[e].rg, h[1]);
+            sx[e] *= rstd;
+        }
+        const float inv_n = 1.f / ((float)s.HW * (float)s.Cg);
+        group_sums<2>(h, sh, s, my);
+        // dx = rstd (g gamma - sum (g gamma) / N - d rstd sum (g gamma d rstd) / N), d = x - mean, rstd gamma = rg
+        const float s0 = h[0] * inv_n, s1 = h[1] * inv_n * rstd * rstd;
+        typename elem<DT>::type* pq = dx + (b * s.HW) * ld_dx + c0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int r = row + k * s.rows_par;
+            if (on && r < s.HW) {
+                P q;
+                if constexpr (XL) q = keep[k * blockDim.x];
+                else q = kx[k];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) q.set(e, fmaf(g[k][e], ch[e].rg, -fmaf(q.get(e) - mean, s1, s0)));
+                q.store(pq + (int64_t)r * ld_dx);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
     if (chan) {
-        float* p0 = part + threadIdx.x * VEC;
-        float* p1 = p0 + blockDim.x * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) { p0[e] = sx[e]; p1[e] = sg[e]; }
-        __syncthreads();
-        const int n = s.cv * VEC;
-        for (int i = threadIdx.x; i < 2 * n; i += blockDim.x) {
-            const int k = i / n, c = i - k * n;
-            const float* q = part + k * blockDim.x * VEC + c;
-            float t = 0.f;
-            for (int r = 0; r < s.rows_par; ++r) t += q[r * n];
-            chan[(b * s.C + g0 * s.Cg + c) * 2 + k] = t;
-        }
-    }
-    if (!on) return;
-    typename elem<DT>::type* pq = dx + (b * s.HW) * ld_dx + c0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int r = row + k * s.rows_par;
-        if (r < s.HW) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float xe = vx[k].get(e);
-                const float h = vd[k].get(e) * act_grad<DT>(xe, mean, rstd, ga[e], be[e], act) * ga[e];
-                vd[k].set(e, rstd * (h - s0 - (xe - mean) * rstd * s1));
-            }
-            vd[k].store(pq + (int64_t)r * ld_dx);
-        }
+        __syncthreads();      // x in LDS is read
+        channel_sums<VEC>(sx, sg, reinterpret_cast<float*>(dyn), s, chan + (b * s.C + g0 * s.Cg) * 2);
     }
 }
 
@@ -386,13 +508,28 @@ __global__ __launch_bounds__(256) void gn_fwd_apply(const typename elem<DT>::typ
         rg[e] = stats[g * 2 + 1] * (gamma ? gamma[m.c0 + e] : 1.f);
         be[e] = fmaf(-low[g], rg[e], beta ? beta[m.c0 + e] : 0.f);
     }
+    with_act(act, [&](auto A) {
 #pragma unroll 4
-    for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
-        Pack<DT, VEC> v;
-        v.load(x + (m.b * HW + r) * ld_x + m.c0);
+        for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
+            Pack<DT, VEC> v;
+            v.load(x + (m.b * HW + r) * ld_x + m.c0);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v.set(e, act_of<DT>(fmaf(v.get(e) - mean[e], rg[e], be[e]), act));
-        v.store(y + (m.b * HW + r) * ld_y + m.c0);
+            for (int e = 0; e < VEC; ++e) v.set(e, act_of<DT, decltype(A)::v>(fmaf(v.get(e) - mean[e], rg[e], be[e])));
+            v.store(y + (m.b * HW + r) * ld_y + m.c0);
+        }
+    });
+}
+
+template <int VEC>
+__device__ __forceinline__ void norms(Norm1* ch, const SplitMap<VEC>& m, int Cg, int G, const float* stats, const float* gamma,
+                                      const float* beta) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int64_t g = m.b * G + (m.c0 + e) / Cg;
+        ch[e].mean = stats[g * 2];
+        ch[e].rstd = stats[g * 2 + 1];
+        ch[e].beta = beta ? beta[m.c0 + e] : 0.f;
+        ch[e].rg = gamma ? ch[e].rstd * gamma[m.c0 + e] : ch[e].rstd;
     }
 }
 
@@ -407,28 +544,25 @@ __global__ __launch_bounds__(256) void gn_bwd_partial(const typename elem<DT>::t
     const int Cg = C / G;
     float sx[VEC] = {}, sg[VEC] = {};
     if (m.on) {
-        float mean[VEC], rstd[VEC], ga[VEC], be[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const int64_t g = m.b * G + (m.c0 + e) / Cg;
-            mean[e] = stats[g * 2];
-            rstd[e] = stats[g * 2 + 1];
-            ga[e] = gamma ? gamma[m.c0 + e] : 1.f;
-            be[e] = beta ? beta[m.c0 + e] : 0.f;
-        }
+        Norm1 ch[VEC];
+        norms<VEC>(ch, m, Cg, G, stats, gamma, beta);
+        with_act(act, [&](auto A) {
 #pragma unroll 2
-        for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
-            Pack<DT, VEC> vx, vd;
-            vx.load(x + (m.b * HW + r) * ld_x + m.c0);
-            vd.load(dy + (m.b * HW + r) * ld_dy + m.c0);
+            for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
+                Pack<DT, VEC> vx, vd;
+                vx.load(x + (m.b * HW + r) * ld_x + m.c0);
+                vd.load(dy + (m.b * HW + r) * ld_dy + m.c0);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float xe = vx.get(e);
-                const float g = vd.get(e) * act_grad<DT>(xe, mean[e], rstd[e], ga[e], be[e], act);
-                sg[e] += g;
-                sx[e] = fmaf(g, (xe - mean[e]) * rstd[e], sx[e]);
+                for (int e = 0; e < VEC; ++e) {
+                    const float xe = vx.get(e), d = xe - ch[e].mean;
+                    const float g = vd.get(e) * act_grad<DT, decltype(A)::v>(xe, d, ch[e], gamma ? gamma + m.c0 + e : nullptr);
+                    sg[e] += g;
+                    sx[e] = fmaf(g, d, sx[e]);
+                }
             }
-        }
+        });
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sx[e] *= ch[e].rstd;
     }
     split_store<VEC>(sx, sg, red, m, C, slots);
 }
@@ -481,30 +615,30 @@ __global__ __launch_bounds__(256) void gn_bwd_apply(const typename elem<DT>::typ
     const SplitMap<VEC> m(HW, C);
     if (!m.on) return;
     const int Cg = C / G;
-    float mean[VEC], rstd[VEC], ga[VEC], be[VEC], s0[VEC], s1[VEC];
+    Norm1 ch[VEC];
+    float s0[VEC], s1[VEC];
+    norms<VEC>(ch, m, Cg, G, stats, gamma, beta);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
         const int64_t g = m.b * G + (m.c0 + e) / Cg;
-        mean[e] = stats[g * 2];
-        rstd[e] = stats[g * 2 + 1];
-        s0[e] = grp[g * 2];
-        s1[e] = grp[g * 2 + 1];
-        ga[e] = gamma ? gamma[m.c0 + e] : 1.f;
-        be[e] = beta ? beta[m.c0 + e] : 0.f;
+        s0[e] = grp[g * 2] * ch[e].rstd;
+        s1[e] = grp[g * 2 + 1] * ch[e].rstd * ch[e].rstd;
     }
+    with_act(act, [&](auto A) {
 #pragma unroll 2
-    for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
-        Pack<DT, VEC> vx, vd;
-        vx.load(x + (m.b * HW + r) * ld_x + m.c0);
-        vd.load(dy + (m.b * HW + r) * ld_dy + m.c0);
+        for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
+            Pack<DT, VEC> vx, vd;
+            vx.load(x + (m.b * HW + r) * ld_x + m.c0);
+            vd.load(dy + (m.b * HW + r) * ld_dy + m.c0);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float xe = vx.get(e);
-            const float h = vd.get(e) * act_grad<DT>(xe, mean[e], rstd[e], ga[e], be[e], act) * ga[e];
-            vd.set(e, rstd[e] * (h - s0[e] - (xe - mean[e]) * rstd[e] * s1[e]));
+            for (int e = 0; e < VEC; ++e) {
+                const float xe = vx.get(e), d = xe - ch[e].mean;
+                const float g = vd.get(e) * act_grad<DT, decltype(A)::v>(xe, d, ch[e], gamma ? gamma + m.c0 + e : nullptr);
+                vd.set(e, fmaf(g, ch[e].rg, -fmaf(d, s1[e], s0[e])));
+            }
+            vd.store(dx + (m.b * HW + r) * ld_dx + m.c0);
         }
-        vd.store(dx + (m.b * HW + r) * ld_dx + m.c0);
-    }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
@@ -536,8 +670,8 @@ inline int gn_vec(int dt, int run, const void* const* ptrs, const int* lds, int 
 
 struct GnPlan { bool resident; int threads, K; GnShape s; };
 
-// vectors of `vec` elements a thread may hold per tensor
-inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax) {
+// kmax: vectors of `vec` elements a thread may hold; tmax: threads of a workgroup
+inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax, int tmax) {
     GnPlan p = {};
     const int Cg = C / G, es = elem_bytes(dt);
     p.s.HW = HW; p.s.C = C; p.s.G = G; p.s.Cg = Cg;
@@ -545,16 +679,17 @@ inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax) {
     for (int d = 1; d <= G; ++d) {
         if (G % d) continue;
         const int64_t cv = (int64_t)d * Cg / vec;
-        if (cv > 1024) break;
-        if (cdiv(HW, 1024 / cv) > kmax) break;                                          // does not fit the registers
-        if (gc && (int64_t)gc * Cg * es >= 64 && (int64_t)gc * Cg * es * HW >= 8192) break;   // wide enough already
-        if (gc && (int64_t)B * G / d < 256) break;                                       // keep a workgroup per CU
+        if (cv > tmax) break;
+        if (cdiv(HW, tmax / cv) > kmax) break;                                           // does not fit the registers
+        // 64 bytes of a pixel and 8 KB in all are enough (32 x 64 x 64 x 256 f16: 31 us with 32, 30 with 64)
+        if (gc && (int64_t)gc * Cg * es >= 64 && (int64_t)gc * Cg * es * HW >= 8192) break;
+        if (gc && (int64_t)B * G / d < 256) break;      // a workgroup for every CU comes before width (one document: 25 against 31 us)
         gc = d;
     }
     if (!gc) return p;
     const int64_t cv = (int64_t)gc * Cg / vec;
     int64_t t = cdiv(cdiv((int64_t)HW * cv, 4), 64) * 64;      // about four vectors a thread
-    if (t > 1024) t = 1024;
+    if (t > tmax) t = tmax;
     if (t < cv) t = cdiv(cv, 64) * 64;
     if (t < 64) t = 64;
     p.threads = (int)t;
@@ -563,6 +698,8 @@ inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax) {
     p.s.rows_par = (int)(t / cv);
     p.s.items = (int64_t)B * (G / gc);
     p.K = (int)cdiv(HW, p.s.rows_par);
+    auto pow2 = [](int64_t v) { return v <= 64 && (v & (v - 1)) == 0; };
+    p.s.fast = pow2(cv) && pow2(cv / gc);
     p.resident = p.K <= kmax && p.s.items <= (1 << 30);
     return p;
 }
@@ -578,7 +715,7 @@ inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax) {
         else { constexpr int VEC = 1; __VA_ARGS__; }                          \
     }
 
-constexpr int GN_FWD_KMAX = 16, GN_BWD_KMAX = 8;
+constexpr int GN_FWD_KMAX = 16;
 
 struct GnSpace { size_t slots, low, chan, grp, total; };
 inline GnSpace gn_space(int B, int HW, int C, int G) {
@@ -623,7 +760,7 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
     const void* ptrs[2] = {x, y};
     const int lds[2] = {ld_x, ld_y};
     const int vec = gn_vec(dtype, C / groups, ptrs, lds, 2);
-    const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX);
+    const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX, 1024);
     if (p.resident) {
         const dim3 grid((unsigned)(cdiv(p.s.items, 8) * 8));
         CUTIE_DISPATCH_DTYPE(dtype, DT, {
@@ -689,22 +826,29 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
         const void* ptrs[3] = {dy, x, dx};
         const int lds[3] = {ld_dy, ld_x, ld_dx};
         const int vec = gn_vec(dtype, C / groups, ptrs, lds, 3);
-        const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_BWD_KMAX);
+        const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, vec > 1 ? 16 : 24, vec > 1 ? 512 : 1024);
         if (p.resident) {
             const dim3 grid((unsigned)(cdiv(p.s.items, 8) * 8));
-            const size_t lds_bytes = params ? (size_t)2 * p.threads * vec * sizeof(float) : 0;
+            const size_t sums = params ? (size_t)2 * p.threads * vec * sizeof(float) : 0;
             CUTIE_DISPATCH_DTYPE(dtype, DT, {
                 typedef typename elem<DT>::type E;
                 GN_VECS(DT, vec, VEC, {
                     int rc = CUTIE_OK;
-                    auto go = [&](auto kern) {
-                        if (lds_bytes) rc = ensure_dyn_lds((const void*)kern, (int)lds_bytes);
+                    auto go = [&](auto kern, int K) {
+                        const size_t held = VEC > 1 ? (size_t)K * p.threads * VEC * sizeof(E) : 0, lds = held > sums ? held : sums;
+                        if (lds) rc = ensure_dyn_lds((const void*)kern, (int)lds);
                         if (rc == CUTIE_OK)
-                            hipLaunchKernelGGL(kern, grid, dim3(p.threads), lds_bytes, stream, (const E*)dy, ld_dy, (const E*)x, ld_x,
-                                               gamma, beta, act, stats, (E*)dx, ld_dx, params ? chan : nullptr, p.s);
+                            hipLaunchKernelGGL(kern, grid, dim3(p.threads), lds, stream, (const E*)dy, ld_dy, (const E*)x, ld_x, gamma, beta,
+                                               act, stats, (E*)dx, ld_dx, params ? chan : nullptr, p.s);
                     };
-                    if (p.K <= 4) go(gn_bwd_resident<DT, VEC, 4>);
-                    else go(gn_bwd_resident<DT, VEC, 8>);
+                    if constexpr (VEC > 1) {
+                        if (p.K <= 4) go(gn_bwd_resident<DT, VEC, 4>, 4);
+                        else if (p.K <= 8) go(gn_bwd_resident<DT, VEC, 8>, 8);
+                        else go(gn_bwd_resident<DT, VEC, 16>, 16);
+                    } else {
+                        if (p.K <= 8) go(gn_bwd_resident<DT, VEC, 8>, 8);
+                        else go(gn_bwd_resident<DT, VEC, 24>, 24);
+                    }
                     if (rc != CUTIE_OK) return rc;
                 })
             });
