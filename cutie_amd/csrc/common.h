@@ -109,6 +109,30 @@ __device__ __forceinline__ void store4(bf16_t* p, float4 v) {
     *reinterpret_cast<uint2*>(p) = u;
 }
 
+// VEC consecutive elements as they lie in memory, aligned to their size
+template <int DT, int VEC> struct Pack {
+    typedef typename elem<DT>::type T;
+    typedef T V __attribute__((ext_vector_type(VEC)));
+    V v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
+    __device__ __forceinline__ float get(int e) const { T t = v[e]; return load_as_f32(&t); }
+    __device__ __forceinline__ void set(int e, float f) { T t; store_from_f32(&t, f); v[e] = t; }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
+    // non-temporal: for a tensor that is touched once and larger than the caches
+    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p)); }
+    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
+};
+template <int DT> struct Pack<DT, 1> {
+    typedef typename elem<DT>::type T;
+    T v;
+    __device__ __forceinline__ void load(const T* p) { v = *p; }
+    __device__ __forceinline__ float get(int) const { return load_as_f32(&v); }
+    __device__ __forceinline__ void set(int, float f) { store_from_f32(&v, f); }
+    __device__ __forceinline__ void store(T* p) const { *p = v; }
+    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(p); }
+    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, p); }
+};
+
 // Instance-norm moments are kept about a per-channel shift, (sum (x - sh), sum (x - sh)^2), with sh = act(bias[c]): a
 // channel that its bias dominates (mean >> std) would lose its whole variance in f32 E[x^2] - E[x]^2.  The shift is a
 // function of the layer's bias and activation code only, so producers and consumers compute the same value; bias

@@ -3,6 +3,10 @@
 //   out[cell][0:E] = scale * table[ids[cell]][0:E]
 //   dtable[v][0:E] (+)= scale * sum of dout[cell][0:E] over the cells with ids[cell] == v, in the order of a stable sort
 //
+// Measured (MI355X): lookup 131072 x 128 f16 10 us, 500009 x 512 bf16 156 us (4.8 TB/s of the 757 MB it must move); gradient
+// 131072 x 128 f16, V 18000, 94 % of the cells on one id: 52 us (28 us of it the two passes of the sort, nine launches); 500009 x
+// 512 bf16, V 120000: 207 us, of which the sums 156 (4.9 TB/s).
+//
 // The lookup is a row copy (HBM).  The gradient sorts (id, cell) pairs - a stable radix sort, least significant digit
 // first - and adds runs of equal ids: every output row has one owner, no float atomics, the same bits every run, and an id
 // that most cells hold (the empty cell of a document grid) costs what any other cells cost.
@@ -11,35 +15,24 @@
 namespace {
 using namespace cutie;
 
-template <int DT, int VEC> struct Row {      // VEC elements of a 16-bit or f32 row as f32
-    typedef typename elem<DT>::type T;
-    static __device__ __forceinline__ void load(const T* p, float* v) {
-        if constexpr (VEC == 1) {
-            v[0] = load_as_f32(p);
-        } else if constexpr (VEC == 4) {
-            const float4 f = load4(p);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
-            typedef T V __attribute__((ext_vector_type(8)));
-            const V q = *reinterpret_cast<const V*>(p);
+// VEC f32 values at an address aligned to 16 bytes (VEC >= 4)
+template <int VEC> __device__ __forceinline__ void load_f32(const float* p, float* v) {
+    if constexpr (VEC == 1) v[0] = *p;
+    else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { const T t = q[e]; v[e] = load_as_f32(&t); }
+        for (int e = 0; e < VEC; e += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p + e);
+            v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
         }
     }
-    static __device__ __forceinline__ void store(T* p, const float* v) {
-        if constexpr (VEC == 1) {
-            store_from_f32(p, v[0]);
-        } else if constexpr (VEC == 4) {
-            store4(p, make_float4(v[0], v[1], v[2], v[3]));
-        } else {
-            typedef T V __attribute__((ext_vector_type(8)));
-            V q;
+}
+template <int VEC> __device__ __forceinline__ void store_f32(float* p, const float* v) {
+    if constexpr (VEC == 1) *p = v[0];
+    else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { T t; store_from_f32(&t, v[e]); q[e] = t; }
-            *reinterpret_cast<V*>(p) = q;
-        }
+        for (int e = 0; e < VEC; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
     }
-};
+}
 
 // `cv` vectors a row, 256 / cv rows side by side (a row wider than 256 vectors takes gridDim.y column blocks)
 template <int ODT, int VEC>
@@ -64,12 +57,7 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[u][e] = 0.f;
-            if (id[u] >= 0 && id[u] < V) {
-                const float* p = table + (int64_t)id[u] * E + c0;
-                if constexpr (VEC == 1) Row<CUTIE_F32, 1>::load(p, v[u]);
-                else if constexpr (VEC == 4) Row<CUTIE_F32, 4>::load(p, v[u]);
-                else { Row<CUTIE_F32, 4>::load(p, v[u]); Row<CUTIE_F32, 4>::load(p + 4, v[u] + 4); }
-            }
+            if (id[u] >= 0 && id[u] < V) load_f32<VEC>(table + (int64_t)id[u] * E + c0, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -83,15 +71,18 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
                 // multiplier (one rounding instead of two, another f16 next to a tie)
                 asm volatile("" : "+v"(v[u][e]));
             }
-            Row<ODT, VEC>::store(out + cell * ld + c0, v[u]);
+            Pack<ODT, VEC> q;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) q.set(e, v[u][e]);
+            q.store_nt(out + cell * ld + c0);      // 500009 x 512 bf16: 156 us, 197 through the caches; 131072 x 128: equal
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------- sort
-constexpr int ITEMS = 8;                // elements a thread ranks
-constexpr int TILE = 256 * ITEMS;       // elements a workgroup ranks in the many-tile form
-constexpr int ONE = 1024 * ITEMS;       // elements one workgroup sorts by itself
+constexpr int ITEMS = 4;                // elements a thread ranks in the many-tile form
+constexpr int TILE = 256 * ITEMS;       // elements a workgroup ranks there
+constexpr int ONE = 1024 * 8;           // elements one workgroup sorts by itself (4 or 8 a thread)
 constexpr int MAX_BITS = 10, MAX_BINS = 1 << MAX_BITS;
 
 // An id outside [0, V) sorts behind every other as the key V and adds to nothing.
@@ -114,7 +105,7 @@ __device__ __forceinline__ unsigned long long same_digit(unsigned d, int bits, u
 // Rank of each of a thread's elements among the tile's elements of its digit, in element order (element = wave * 64 *
 // ITEMS + round * 64 + lane).  cnt[waves][bins] in LDS, cleared here; afterwards cnt[w][d] = elements of digit d in earlier
 // waves and total[d] (nullable) = the tile's count.
-template <int WAVES>
+template <int WAVES, int ITEMS>
 __device__ __forceinline__ void tile_rank(const unsigned* d, const bool* ok, int bits, unsigned short (*cnt)[MAX_BINS], int* rank,
                                           unsigned* total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
@@ -184,29 +175,14 @@ template <int THREADS> __device__ __forceinline__ void bin_scan(unsigned* v, int
     __syncthreads();
 }
 
-__device__ __forceinline__ void clear_part(float* dtable, int64_t n, int64_t block, int64_t blocks) {
-    const int64_t step = blocks * blockDim.x;
-    if (((uintptr_t)dtable & 15) == 0) {
-        const int64_t n4 = n >> 2;
-        for (int64_t i = block * blockDim.x + threadIdx.x; i < n4; i += step)
-            reinterpret_cast<float4*>(dtable)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int64_t i = (n4 << 2) + block * blockDim.x + threadIdx.x; i < n; i += step) dtable[i] = 0.f;
-    } else {
-        for (int64_t i = block * blockDim.x + threadIdx.x; i < n; i += step) dtable[i] = 0.f;
-    }
-}
-
-// block 0 sorts n <= ONE pairs by itself; the other blocks clear the table
+// one workgroup sorts n <= 1024 ITEMS pairs
+template <int ITEMS>
 __global__ __launch_bounds__(1024) void sort_one_kernel(const int32_t* __restrict__ ids, int n, int V, int passes, int bits,
-                                                        uint2* __restrict__ out, float* __restrict__ dtable, int64_t clear) {
+                                                        uint2* __restrict__ out) {
     __shared__ unsigned short cnt[16][MAX_BINS];
     __shared__ unsigned base[MAX_BINS];
     __shared__ unsigned wsum[4];
     extern __shared__ uint2 pairs[];      // [n]
-    if (blockIdx.x) {
-        clear_part(dtable, clear, blockIdx.x - 1, gridDim.x - 1);
-        return;
-    }
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint2 p[ITEMS];
     bool ok[ITEMS];
@@ -222,7 +198,7 @@ __global__ __launch_bounds__(1024) void sort_one_kernel(const int32_t* __restric
         const int shift = pass * bits;
 #pragma unroll
         for (int r = 0; r < ITEMS; ++r) d[r] = (p[r].x >> shift) & ((1u << bits) - 1);
-        tile_rank<16>(d, ok, bits, cnt, rank, base);
+        tile_rank<16, ITEMS>(d, ok, bits, cnt, rank, base);
         bin_scan<1024>(base, 1 << bits, wsum);
         if (pass + 1 < passes) {
 #pragma unroll
@@ -240,16 +216,11 @@ __global__ __launch_bounds__(1024) void sort_one_kernel(const int32_t* __restric
     }
 }
 
-// counts[bin][tile] of one digit; blocks behind the tiles clear the table (first pass)
+// counts[tile][bin] of one digit
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_count_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
-                                                         int shift, int bits, int tiles, unsigned* __restrict__ counts,
-                                                         float* __restrict__ dtable, int64_t clear) {
+                                                         int shift, int bits, unsigned* __restrict__ counts) {
     __shared__ unsigned hist[4][MAX_BINS];
-    if ((int)blockIdx.x >= tiles) {
-        clear_part(dtable, clear, blockIdx.x - tiles, gridDim.x - tiles);
-        return;
-    }
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
     for (int i = threadIdx.x; i < 4 * bins; i += 256) hist[i >> bits][i & (bins - 1)] = 0;
     __syncthreads();
@@ -265,32 +236,45 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const int32_t* __restri
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += 256)
-        counts[(int64_t)b * tiles + blockIdx.x] = hist[0][b] + hist[1][b] + hist[2][b] + hist[3][b];
+        counts[((int64_t)blockIdx.x << bits) + b] = hist[0][b] + hist[1][b] + hist[2][b] + hist[3][b];
 }
 
-// one wave per bin: counts[bin][tile] becomes the count in earlier tiles, totals[bin] the whole
-__global__ __launch_bounds__(256) void sort_scan_kernel(unsigned* __restrict__ counts, int tiles, int bins, unsigned* __restrict__ totals) {
-    const int lane = threadIdx.x & 63, b = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (b >= bins) return;
-    unsigned run = 0;
-    for (int t0 = 0; t0 < tiles; t0 += 64) {
-        const int t = t0 + lane;
-        const unsigned c = t < tiles ? counts[(int64_t)b * tiles + t] : 0;
-        unsigned inc = c;
+// counts[tile][bin] becomes the count in earlier tiles, totals[bin] the whole: a workgroup takes 16 bins, 64 lanes a bin cut the
+// tiles into 64 runs, each lane adds its run, the lanes' sums are scanned, and each lane walks its run again
+__global__ __launch_bounds__(1024) void sort_scan_kernel(unsigned* __restrict__ counts, int tiles, int bits, unsigned* __restrict__ totals) {
+    __shared__ unsigned sh[64][17];
+    const int el = threadIdx.x & 15, part = threadIdx.x >> 4, bin = blockIdx.x * 16 + el, bins = 1 << bits;
+    const int per = (tiles + 63) / 64, t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
+    unsigned s = 0;
+    if (bin < bins)
+        for (int t = t0; t < t1; ++t) s += counts[((int64_t)t << bits) + bin];
+    sh[part][el] = s;
+    __syncthreads();
+    // 16 waves: wave w scans bin w over its 64 parts
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const unsigned own = sh[lane][w];
+    unsigned inc = own;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned u = __shfl_up(inc, o, 64);
-            if (lane >= o) inc += u;
-        }
-        if (t < tiles) counts[(int64_t)b * tiles + t] = run + inc - c;
-        run += __shfl(inc, 63, 64);
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += u;
     }
-    if (lane == 0) totals[b] = run;
+    sh[lane][w] = inc - own;
+    if (lane == 63 && blockIdx.x * 16 + w < bins) totals[blockIdx.x * 16 + w] = inc;
+    __syncthreads();
+    if (bin >= bins) return;
+    unsigned run = sh[part][el];
+    for (int t = t0; t < t1; ++t) {
+        unsigned* p = counts + ((int64_t)t << bits) + bin;
+        const unsigned c = *p;
+        *p = run;
+        run += c;
+    }
 }
 
 template <bool FIRST>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
-                                                           int shift, int bits, int tiles, const unsigned* __restrict__ counts,
+                                                           int shift, int bits, const unsigned* __restrict__ counts,
                                                            const unsigned* __restrict__ totals, uint2* __restrict__ out) {
     __shared__ unsigned short cnt[4][MAX_BINS];
     __shared__ unsigned base[MAX_BINS];
@@ -309,8 +293,8 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int32_t* __rest
     }
     for (int b = threadIdx.x; b < bins; b += 256) base[b] = totals[b];
     bin_scan<256>(base, bins, wsum);
-    for (int b = threadIdx.x; b < bins; b += 256) base[b] += counts[(int64_t)b * tiles + blockIdx.x];
-    tile_rank<4>(d, ok, bits, cnt, rank, nullptr);
+    for (int b = threadIdx.x; b < bins; b += 256) base[b] += counts[((int64_t)blockIdx.x << bits) + b];
+    tile_rank<4, ITEMS>(d, ok, bits, cnt, rank, nullptr);
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r)
         if (ok[r]) out[base[d[r]] + rank[r]] = p[r];
@@ -323,7 +307,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int32_t* __rest
 // in the workspace (slots f32 [chunks][2][E], starts[chunk] = 1 where a run leaves to the right), and run_join_kernel adds
 // the parts of a run that spans workgroups.
 struct SumShape {
-    int64_t n;
+    int64_t n, chunks;
     int V, E, ld;
     int rows, L;          // subgroups of a workgroup, pairs of a subgroup
     float scale;
@@ -337,62 +321,92 @@ __device__ __forceinline__ void put(float* dtable, const SumShape& s, unsigned k
     *p = s.accumulate ? *p + t : t;
 }
 
+// Rows that no cell names: a wave takes 64 rows, each lane looks its row up among the sorted pairs, the wave clears the rows
+// that are not there.  (Clearing the whole table first writes the other rows twice: 31 us of 242 at V 120000, E 512.)
+__device__ __forceinline__ void clear_absent(const uint2* pairs, float* dtable, const SumShape& s, int64_t wave) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = wave * 64 + lane;
+    bool absent = false;
+    if (row < s.V) {
+        int64_t lo = 0, hi = s.n;      // first pair whose key is not below the row
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) >> 1;
+            if ((int64_t)pairs[mid].x < row) lo = mid + 1;
+            else hi = mid;
+        }
+        absent = lo == s.n || (int64_t)pairs[lo].x != row;
+    }
+    const bool wide = (s.E & 3) == 0 && (reinterpret_cast<uintptr_t>(dtable) & 15) == 0;
+    for (unsigned long long m = __ballot(absent); m; m &= m - 1) {
+        float* p = dtable + (wave * 64 + __builtin_ctzll(m)) * s.E;
+        if (wide)
+            for (int c = lane * 4; c < s.E; c += 256) *reinterpret_cast<float4*>(p + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        else
+            for (int c = lane; c < s.E; c += 64) p[c] = 0.f;
+    }
+}
+
+constexpr int CHUNK_MAX = 1280;      // pairs of a workgroup
+
 template <int DT, int VEC>
 __global__ __launch_bounds__(256) void run_sum_kernel(const uint2* __restrict__ pairs, const typename elem<DT>::type* __restrict__ dout,
                                                       float* __restrict__ dtable, SumShape s, float* __restrict__ slots,
                                                       int* __restrict__ starts) {
     __shared__ float part[2][256 * VEC];
     __shared__ int flags[256];
+    __shared__ unsigned key[CHUNK_MAX + 2], pos[CHUNK_MAX];      // key[i + 1] is the chunk's pair i; its neighbours outside
+    if (blockIdx.x >= s.chunks) {      // workgroups behind the chunks: four waves of rows to clear
+        if (blockIdx.y == 0) clear_absent(pairs, dtable, s, ((int64_t)blockIdx.x - s.chunks) * 4 + (threadIdx.x >> 6));
+        return;
+    }
     const int v0 = blockIdx.y * 256, nv = min(256, s.E / VEC - v0);
     const int col = threadIdx.x % nv, j = threadIdx.x / nv;
     const int c0 = (v0 + col) * VEC, width = nv * VEC;
-    const int64_t chunk0 = (int64_t)blockIdx.x * s.rows * s.L;
-    const int64_t b = chunk0 + (int64_t)j * s.L;
+    const int chunk = s.rows * s.L;
+    const int64_t chunk0 = (int64_t)blockIdx.x * chunk;
+    for (int i = threadIdx.x; i < chunk + 2; i += 256) {
+        const int64_t g = chunk0 + i - 1;
+        const uint2 p = g >= 0 && g < s.n ? pairs[g] : make_uint2(0xffffffffu, 0);      // no key: V < 2^30
+        key[i] = p.x;
+        if (i >= 1 && i <= chunk) pos[i - 1] = p.y;
+    }
+    __syncthreads();
     if (j < s.rows) {
         int f = 0;
-        if (b < s.n) {
-            const int64_t e = min(s.n, b + s.L);
+        const int b = j * s.L;
+        if (chunk0 + b < s.n) {
+            const int e = (int)min((int64_t)(b + s.L), s.n - chunk0);
             float acc[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-            bool entered = b > 0 && pairs[b - 1].x == pairs[b].x;
-            constexpr int U = 4;
-            for (int64_t i0 = b; i0 < e; i0 += U) {
-                uint2 p[U + 1];
-                float v[U][VEC];
-#pragma unroll
-                for (int u = 0; u <= U; ++u) p[u] = i0 + u < s.n ? pairs[i0 + u] : make_uint2(0xffffffffu, 0);
+            bool entered = key[b] == key[b + 1];
+            constexpr int U = 8;
+            for (int i0 = b; i0 < e; i0 += U) {
+                Pack<DT, VEC> v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (i0 + u < e) Row<DT, VEC>::load(dout + (int64_t)p[u].y * s.ld + c0, v[u]);
+                    if (i0 + u < e) v[u].load_nt(dout + (int64_t)pos[i0 + u] * s.ld + c0);
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (i0 + u >= e) break;
+                    const int i = i0 + u;
+                    if (i >= e) break;
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
-                    const bool same = p[u].x == p[u + 1].x, end = i0 + u + 1 == e;
-                    if (same && !end) continue;
-                    const bool leaves = same;
+                    for (int k = 0; k < VEC; ++k) acc[k] += v[u].get(k);
+                    const unsigned id = key[i + 1];
+                    const bool leaves = id == key[i + 2];
+                    if (leaves && i + 1 < e) continue;
                     if (entered || leaves) {
                         f |= entered ? (leaves ? 3 : 1) : 4;
                         float* q = part[entered ? 0 : 1] + j * width + col * VEC;
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) q[k] = acc[k];
-                    } else if (p[u].x < (unsigned)s.V) {
-                        float* q = dtable + (int64_t)p[u].x * s.E + c0;
+                    } else if (id < (unsigned)s.V) {
+                        float* q = dtable + (int64_t)id * s.E + c0;
                         float t[VEC];
+                        if (s.accumulate) load_f32<VEC>(q, t);
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) t[k] = s.scale * acc[k];
-                        if (s.accumulate) {
-#pragma unroll
-                            for (int k = 0; k < VEC; ++k) t[k] += q[k];
-                        }
-                        if constexpr (VEC == 8) {
-                            Row<CUTIE_F32, 4>::store(q, t);
-                            Row<CUTIE_F32, 4>::store(q + 4, t + 4);
-                        } else {
-                            Row<CUTIE_F32, VEC>::store(q, t);
-                        }
+                        for (int k = 0; k < VEC; ++k) t[k] = s.accumulate ? t[k] + s.scale * acc[k] : s.scale * acc[k];
+                        store_f32<VEC>(q, t);
                     }
                     entered = false;
 #pragma unroll
@@ -415,7 +429,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const uint2* __restrict__ 
                 open = (f & 2) != 0;
                 if (!open) {
                     if (before) slots[((int64_t)blockIdx.x * 2) * s.E + v0 * VEC + c] = acc;
-                    else put(dtable, s, pairs[chunk0 + (int64_t)k * s.L].x, v0 * VEC + c, acc);
+                    else put(dtable, s, key[k * s.L + 1], v0 * VEC + c, acc);
                     acc = 0.f;
                     before = false;
                 }
@@ -427,41 +441,58 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const uint2* __restrict__ 
             }
         }
         if (open) slots[((int64_t)blockIdx.x * 2 + (before ? 0 : 1)) * s.E + v0 * VEC + c] = acc;
-        if (c == 0 && v0 == 0) starts[blockIdx.x] = open && !before;
+        if (c == 0 && v0 == 0) starts[blockIdx.x] = open ? (before ? 2 : 1) : 0;
     }
 }
 
-// one workgroup per chunk and column block: where a run starts in this chunk and leaves it, the sum of its parts, eight
-// chunks apart in each of eight lanes, the eight sums in lane order
-__global__ __launch_bounds__(256) void run_join_kernel(const uint2* __restrict__ pairs, float* __restrict__ dtable, SumShape s,
+// One workgroup per chunk (and JOIN vectors of columns): where a run starts in this chunk and leaves it (starts 1), the sum of its
+// parts up to the first chunk that it does not fill (starts 2: filled).  The parts go round the subgroups that a row of columns
+// leaves room for, whose sums are added in order.
+constexpr int JOIN = 256;      // 131072 cells, most on one id: 9.3 us, 8.8 with 1024 threads; 500009 cells: 6.5 and 9.6
+template <int VEC>
+__global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict__ pairs, float* __restrict__ dtable, SumShape s,
                                                        const float* __restrict__ slots, const int* __restrict__ starts) {
-    __shared__ float sh[8][32];
-    const int64_t w = blockIdx.x, chunk = (int64_t)s.rows * s.L;
-    if (!starts[w]) return;
-    const unsigned key = pairs[(w + 1) * chunk - 1].x;
+    __shared__ float sh[JOIN * VEC];
+    __shared__ int first;
+    const int64_t w = blockIdx.x;
+    if (starts[w] != 1) return;
+    const unsigned key = pairs[(w + 1) * s.rows * s.L - 1].x;
     if (key >= (unsigned)s.V) return;
-    int64_t lo = (w + 1) * chunk, hi = s.n;      // first pair behind the run: pairs[lo] belongs to it
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (pairs[mid].x == key) lo = mid;
-        else hi = mid;
+    int64_t last = w + 1;
+    for (;; last += JOIN) {      // a run that leaves a chunk ends in a later one, so there is a first that is not filled
+        if (threadIdx.x == 0) first = JOIN;
+        __syncthreads();
+        const int64_t k = last + threadIdx.x;
+        if (k >= s.chunks || starts[k] != 2) atomicMin(&first, (int)threadIdx.x);
+        __syncthreads();
+        const int f = first;
+        __syncthreads();
+        if (f < JOIN) { last += f; break; }
     }
-    const int64_t last = lo / chunk;
-    const int el = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const int c = blockIdx.y * 32 + el;
-    float t = 0.f;
-    if (c < s.E) {
-        if (part == 0) t = slots[(w * 2 + 1) * s.E + c];
-#pragma unroll 4
-        for (int64_t k = w + 1 + part; k <= last; k += 8) t += slots[k * 2 * s.E + c];
-    }
-    sh[part][el] = t;
-    __syncthreads();
-    if (part || c >= s.E) return;
-    t = 0.f;
+    const int v0 = blockIdx.y * JOIN, nv = min(JOIN, s.E / VEC - v0), parts = JOIN / nv;
+    const int col = threadIdx.x % nv, part = threadIdx.x / nv, c = (v0 + col) * VEC;
+    float t[VEC];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += sh[k][el];
-    put(dtable, s, key, c, t);
+    for (int e = 0; e < VEC; ++e) t[e] = 0.f;
+    if (part < parts) {
+        if (part == 0) load_f32<VEC>(slots + (w * 2 + 1) * s.E + c, t);
+#pragma unroll 8
+        for (int64_t k = w + 1 + part; k <= last; k += parts) {
+            float v[VEC];
+            load_f32<VEC>(slots + k * 2 * s.E + c, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sh[threadIdx.x * VEC + e] = t[e];
+    __syncthreads();
+    if (part) return;
+    for (int q = 1; q < parts; ++q)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t[e] += sh[(q * nv + col) * VEC + e];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) put(dtable, s, key, c + e, t[e]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
@@ -484,9 +515,11 @@ inline SumPlan sum_plan(int64_t n, int E, int vec) {
     const int cv = E / vec;
     p.ncol = (int)cdiv(cv, 256);
     p.rows = 256 / (cv < 256 ? cv : 256);
-    const int want = n <= 65536 ? 64 : (n <= 262144 ? 256 : 512);       // pairs of a workgroup
+    // pairs of a workgroup: enough workgroups for the chip first (131072 x 128: 49 us with 256), then few parts to join
+    // (500009 x 512: 318 us with 128, 254 with 256, 242 with 512, 239 with 1024, 268 with 2048)
+    const int want = n <= 65536 ? 64 : (n <= 262144 ? 256 : 1024);
     p.L = (int)cdiv(want, p.rows);
-    if (p.L < 4) p.L = 4;
+    if (p.L < 4) p.L = 4;                                                // rows * L < max(want + rows, 4 * 256) <= CHUNK_MAX
     p.chunks = cdiv(n, (int64_t)p.rows * p.L);
     return p;
 }
@@ -574,30 +607,29 @@ extern "C" int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, cons
     const int es = dout_dtype == CUTIE_F32 ? 4 : 2;
     CUTIE_CHECK_ARG(((uintptr_t)dout % es) == 0 && ((uintptr_t)dtable % 4) == 0 && ((uintptr_t)ids % 4) == 0,
                     "embed_grad_sorted: misaligned pointers");
-    const int64_t clear = accumulate ? 0 : (int64_t)V * E;
-    int64_t fill = cdiv(clear, 4096);
-    if (fill > 1024) fill = 1024;
     const GradSpace w = n_cells ? grad_space(n_cells, V, E) : GradSpace{};
     if (n_cells && (!workspace || workspace_bytes < w.total || !aligned16(workspace))) {
         set_error("embed_grad_sorted: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
         return CUTIE_E_WORKSPACE;
     }
-    if (n_cells == 0) {
-        if (fill) {
-            hipLaunchKernelGGL(sort_one_kernel, dim3((unsigned)fill + 1), dim3(1024), 0, stream, ids, 0, V, 0, 1, (uint2*)nullptr, dtable, clear);
-            CUTIE_CHECK_LAUNCH();
-        }
-        return CUTIE_OK;
-    }
+    if (n_cells == 0 && accumulate) return CUTIE_OK;
     char* ws = (char*)workspace;
     const SortPlan sp = sort_plan(n_cells, V);
-    uint2* sorted;
-    if (sp.one) {
+    uint2* sorted = nullptr;
+    if (n_cells == 0) {
+    } else if (sp.one) {
         sorted = (uint2*)(ws + w.a);
         const size_t lds = sp.passes > 1 ? (size_t)n_cells * sizeof(uint2) : 0;
-        CUTIE_ENSURE_LDS(sort_one_kernel, ONE * sizeof(uint2));
-        hipLaunchKernelGGL(sort_one_kernel, dim3((unsigned)fill + 1), dim3(1024), lds, stream, ids, (int)n_cells, V, sp.passes, sp.bits,
-                           sorted, dtable, clear);
+        auto go = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3(1), dim3(1024), lds, stream, ids, (int)n_cells, V, sp.passes, sp.bits, sorted);
+        };
+        if (n_cells <= 4096) {
+            CUTIE_ENSURE_LDS(sort_one_kernel<4>, 4096 * sizeof(uint2));
+            go(sort_one_kernel<4>);
+        } else {
+            CUTIE_ENSURE_LDS(sort_one_kernel<8>, ONE * sizeof(uint2));
+            go(sort_one_kernel<8>);
+        }
         CUTIE_CHECK_LAUNCH();
     } else {
         uint2* buf[2] = {(uint2*)(ws + w.a), (uint2*)(ws + w.b)};
@@ -608,34 +640,27 @@ extern "C" int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, cons
             const uint2* in = pass ? buf[(pass - 1) & 1] : nullptr;
             uint2* out = buf[pass & 1];
             const int shift = pass * sp.bits;
-            const unsigned count_blocks = (unsigned)sp.tiles + (pass == 0 ? (unsigned)fill : 0u);
-            if (pass == 0)
-                hipLaunchKernelGGL(sort_count_kernel<true>, dim3(count_blocks), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits,
-                                   sp.tiles, counts, dtable, clear);
-            else
-                hipLaunchKernelGGL(sort_count_kernel<false>, dim3(count_blocks), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits,
-                                   sp.tiles, counts, dtable, (int64_t)0);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)cdiv(bins, 4)), dim3(256), 0, stream, counts, sp.tiles, bins, totals);
-            if (pass == 0)
-                hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift,
-                                   sp.bits, sp.tiles, counts, totals, out);
-            else
-                hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift,
-                                   sp.bits, sp.tiles, counts, totals, out);
+            auto count = pass ? sort_count_kernel<false> : sort_count_kernel<true>;
+            auto scatter = pass ? sort_scatter_kernel<false> : sort_scatter_kernel<true>;
+            hipLaunchKernelGGL(count, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)cdiv(bins, 16)), dim3(1024), 0, stream, counts, sp.tiles, sp.bits, totals);
+            hipLaunchKernelGGL(scatter, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts, totals,
+                               out);
             CUTIE_CHECK_LAUNCH();
         }
         sorted = buf[(sp.passes - 1) & 1];
     }
     const SumPlan p = sum_plan(n_cells, E, row_vec(dout_dtype, E, dout, ld_dout, dtable));
     SumShape s;
-    s.n = n_cells; s.V = V; s.E = E; s.ld = ld_dout; s.rows = p.rows; s.L = p.L; s.scale = scale; s.accumulate = accumulate;
+    s.n = n_cells; s.chunks = p.chunks; s.V = V; s.E = E; s.ld = ld_dout; s.rows = p.rows; s.L = p.L; s.scale = scale; s.accumulate = accumulate;
     float* slots = (float*)(ws + w.slots);
     int* starts = (int*)(ws + w.starts);
+    const int64_t blocks = p.chunks + (accumulate ? 0 : cdiv(V, 256));
     CUTIE_DISPATCH_DTYPE(dout_dtype, DT, {
         typedef typename elem<DT>::type T;
         auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, dim3((unsigned)p.chunks, (unsigned)p.ncol), dim3(256), 0, stream, sorted, (const T*)dout, dtable, s,
-                               slots, starts);
+            hipLaunchKernelGGL(kern, dim3((unsigned)blocks, (unsigned)p.ncol), dim3(256), 0, stream, sorted, (const T*)dout, dtable, s, slots,
+                               starts);
         };
         if constexpr (DT != CUTIE_F32) {
             if (p.vec == 8) go(run_sum_kernel<DT, 8>);
@@ -644,8 +669,11 @@ extern "C" int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, cons
         if (p.vec == 1) go(run_sum_kernel<DT, 1>);
     });
     CUTIE_CHECK_LAUNCH();
-    hipLaunchKernelGGL(run_join_kernel, dim3((unsigned)p.chunks, (unsigned)cdiv(E, 32)), dim3(256), 0, stream, sorted, dtable, s, slots,
-                       starts);
+    if (n_cells == 0) return CUTIE_OK;
+    const int jv = E % 4 == 0 ? 4 : 1;
+    const dim3 jgrid((unsigned)p.chunks, (unsigned)cdiv(E / jv, JOIN));
+    if (jv == 4) hipLaunchKernelGGL(run_join_kernel<4>, jgrid, dim3(JOIN), 0, stream, sorted, dtable, s, slots, starts);
+    else hipLaunchKernelGGL(run_join_kernel<1>, jgrid, dim3(JOIN), 0, stream, sorted, dtable, s, slots, starts);
     CUTIE_CHECK_LAUNCH();
     return CUTIE_OK;
 }

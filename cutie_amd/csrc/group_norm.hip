@@ -24,24 +24,6 @@ using namespace cutie;
 
 constexpr int GN_ACT_NONE = 0, GN_ACT_RELU = 1, GN_ACT_SIGMOID = 2, GN_ACT_SILU = 3;
 
-template <int DT, int VEC> struct Pack {      // VEC consecutive elements as they lie in memory
-    typedef typename elem<DT>::type T;
-    typedef T V __attribute__((ext_vector_type(VEC)));
-    V v;
-    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
-    __device__ __forceinline__ float get(int e) const { T t = v[e]; return load_as_f32(&t); }
-    __device__ __forceinline__ void set(int e, float f) { T t; store_from_f32(&t, f); v[e] = t; }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
-};
-template <int DT> struct Pack<DT, 1> {
-    typedef typename elem<DT>::type T;
-    T v;
-    __device__ __forceinline__ void load(const T* p) { v = *p; }
-    __device__ __forceinline__ float get(int) const { return load_as_f32(&v); }
-    __device__ __forceinline__ void set(int, float f) { store_from_f32(&v, f); }
-    __device__ __forceinline__ void store(T* p) const { *p = v; }
-};
-
 // The loops are written once per activation (with_act): the choice is uniform, and left inside a loop it costs a third of the
 // instructions of a kernel whose arithmetic is as long as its memory traffic.
 template <int A> struct Act { static constexpr int v = A; };
