@@ -1,6 +1,6 @@
 // K17: the orthogonalised update.
 //
-//   X0 = U / (|U|_F + eps);   X <- X (a I + b A + c A A), A = X^T X   (steps times)
+//   X0 = U / (|U|_F + eps);   X <- X B, B = a I + b A + c A A, A = X^T X   (steps times)
 // maps every singular value s of X0 to a s + b s^3 + c s^5, again and again: the quintic Newton-Schulz iteration with
 // a = 3.4445, b = -4.7750, c = 2.0315, which takes (0, 1] towards 1 (0.68 .. 1.21 after five steps from s >= 1e-2).  The update
 // around it: m' = mu m + g', U = g' + mu m' (or m'), p' = p (1 - lr wd) - lr k X.
@@ -10,8 +10,8 @@
 // 22 bits).  Against f64 the error is that of the f32 computation (2e-6 of the norm after five steps on a 256 x 1920 matrix in
 // both); one f16 or bf16 term instead gives 2e-2, since small singular values are amplified up to 3.4445 ** 5 = 485 times.
 // f16 has no range to spare, so each kind of matrix is kept at a fixed power of two: X (singular values at most 1.21)
-// times 2^12, A (at most 1.47) and B = b A + c A A (at most 2.81 in magnitude) times 2^13: entries stay below 23100, and
-// the smallest step of f16, 2^-24, is 2^-36 of X.
+// times 2^12, A (at most 1.47) and B (at most 3.4445) times 2^13: entries stay below 28300, and the smallest step of f16, 2^-24,
+// is 2^-36 of X.
 //
 // Layout.  L = max(rows, cols) rows of S = min(rows, cols) values, both padded with zeros to multiples of 64 (the transpose of
 // a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
@@ -24,6 +24,7 @@ using namespace cutie::convk;
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float X_SCALE = 4096.f, INV_X_SCALE = 1.f / 4096.f;      // 2^12
+constexpr float AB_SCALE = 8192.f;                                 // 2^13
 constexpr float AB_FROM_XX = 1.f / 2048.f;                         // 2^24 (X^T X) -> 2^13 A
 constexpr float AB_FROM_AA = 1.f / 8192.f;                         // 2^26 (A A)   -> 2^13 A A
 constexpr float X_FROM_XB = 1.f / 8192.f;                          // 2^25 (X B)   -> 2^12 X B
@@ -47,6 +48,12 @@ struct Hyper {
     const int32_t* invalid;
 };
 
+// Workgroups that read the same rows run side by side behind one L2: dispatch deals consecutive blocks to the eight XCDs in turn,
+// so XCD x takes the x-th eighth of the logical ids.
+__device__ __forceinline__ int xcd_id() {
+    const int n = gridDim.x, q = n >> 3, r = n & 7, x = blockIdx.x & 7;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+}
 __device__ __forceinline__ int find(const Starts& s, int n, int id) {
     int i = 0;
     while (i + 1 < n && id >= s.v[i + 1]) ++i;
@@ -57,6 +64,10 @@ __device__ __forceinline__ char* at(char* ws, int off) { return ws + (int64_t)of
 // the step is skipped: a gradient that is not finite, or results marked invalid
 __device__ __forceinline__ bool skip_step(const Hyper& h) {
     return (h.invalid && *h.invalid != 0) || (h.gnorm_sq && !(fabsf(*h.gnorm_sq) <= 3.0e38f));
+}
+
+__device__ __forceinline__ float clip_scale(const Hyper& h) {
+    return h.gnorm_sq && h.clip > 0.f ? h.grad_scale * (h.clip / fmaxf(sqrtf(*h.gnorm_sq) * h.grad_scale, h.clip)) : h.grad_scale;
 }
 
 __device__ __forceinline__ void block_sum_f64(double v, double* out) {
@@ -87,8 +98,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Mats ms, Ios ios, Starts s
         float* u = (float*)at(ws, M.y1);
         const bool skip = skip_step(h);
         const float inv = h.loss_scale ? h.loss_scale[1] : 1.f;
-        float scale = h.grad_scale;
-        if (h.gnorm_sq && h.clip > 0.f) scale *= h.clip / fmaxf(sqrtf(*h.gnorm_sq) * h.grad_scale, h.clip);
+        const float scale = clip_scale(h);
         for (int64_t e = e0 + threadIdx.x; e < e1; e += 256) {
             const float g = (io.g[e] * inv + h.l2 * io.p[e]) * scale;
             const float m0 = io.m[e];
@@ -122,6 +132,12 @@ __device__ __forceinline__ void join4(uint2 hi, uint2 lo, float* v) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (float)h[e] + (float)l[e];
 }
+__device__ __forceinline__ void store4_split(char* q, const float* x) {
+    uint2 hi, lo;
+    split4(x, hi, lo);
+    *reinterpret_cast<uint2*>(q) = hi;
+    *reinterpret_cast<uint2*>(q + 64) = lo;
+}
 // byte offset of value c (a multiple of 4) of a row's hi part; its lo part lies 64 bytes further
 __device__ __forceinline__ int64_t cell(int64_t row, int ld, int c) { return row * ((int64_t)ld * 4) + (c >> 5) * 128 + (c & 31) * 2; }
 
@@ -141,36 +157,59 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
     double s = 0;
     for (int64_t k = threadIdx.x; k < parts; k += 256) s += part[k];
     block_sum_f64(s, &total);
+    if (!flip) {
+        // straight through: 16 lanes take a row of 64, four values each
+        __syncthreads();
+        const float k = (float)((double)X_SCALE / (sqrt(total) + (double)eps));
+        const int c = s0 + (threadIdx.x & 15) * 4;
+        const bool wide = (M.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0 && c < M.cols;
+#pragma unroll
+        for (int r = threadIdx.x >> 4; r < 64; r += 16) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (l0 + r < M.rows) {
+                const float* p = src + (int64_t)(l0 + r) * M.cols + c;
+                if (wide) {
+                    const float4 f = *reinterpret_cast<const float4*>(p);
+                    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < M.cols) v[e] = p[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= k;
+            store4_split(at(ws, M.y0) + cell(l0 + r, M.Sp, c), v);
+        }
+        return;
+    }
     const int c = threadIdx.x & 63;
     for (int r = threadIdx.x >> 6; r < 64; r += 4) {
         // read along the caller's rows
-        const int row = (flip ? s0 : l0) + r, col = (flip ? l0 : s0) + c;
-        const float v = row < M.rows && col < M.cols ? src[(int64_t)row * M.cols + col] : 0.f;
-        if (flip) tile[c][r] = v;
-        else tile[r][c] = v;
+        const int row = s0 + r, col = l0 + c;
+        tile[c][r] = row < M.rows && col < M.cols ? src[(int64_t)row * M.cols + col] : 0.f;
     }
     __syncthreads();
     const float k = (float)((double)X_SCALE / (sqrt(total) + (double)eps));
     const int l = threadIdx.x >> 2, q = (threadIdx.x & 3) * 16;
-    char* out = at(ws, M.y0) + cell(l0 + l, M.Sp, s0 + q);
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
         float v[4];
-        uint2 hi, lo;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = tile[l][q + e + j] * k;
-        split4(v, hi, lo);
-        *reinterpret_cast<uint2*>(out + e * 2) = hi;
-        *reinterpret_cast<uint2*>(out + 64 + e * 2) = lo;
+        store4_split(at(ws, M.y0) + cell(l0 + l, M.Sp, s0 + q + e), v);
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- products
 // Workgroup of 4 waves, 2 x 2, tile T x T with T = 32 F, a wave F x F fragments of 16 x 16.  A K step is 32 values: the tile's
-// 128-byte lines (hi and lo) go to LDS by buffer_load ... lds, two stages, the next one in flight while this one is used.
+// 128-byte lines (hi and lo) go to LDS by buffer_load ... lds, STAGES of them, all but one in flight while that one is used.
 template <int F> struct Shape {
     static constexpr int T = 32 * F, HALF = T * 128, STAGE = 2 * HALF;      // bytes of one operand, of both
-    static constexpr int LDS = 2 * STAGE;
+    // F = 4: two workgroups a CU with two stages (14 filters 475 us, 2048 x 8192 1.82 ms) beat one with three or four (558, 567 us;
+    // 2.28, 2.25 ms).  F = 2: three stages 475 us, two 480, four 475.
+    static constexpr int STAGES = F == 4 ? 2 : 3;
+    static constexpr int LDS = STAGES * STAGE;
     static constexpr int PIECES = T / 8;      // 1-KB pieces of an operand; a wave moves PIECES / 4 of each
 };
 __device__ __forceinline__ int tr_swz(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
@@ -189,17 +228,23 @@ __device__ __forceinline__ void multiply(const Frags<F>& p, const Frags<F>& q, f
         }
 }
 
-// my pieces of the stage have landed and my reads of the other one are done; then everybody's are
-__device__ __forceinline__ void stage_ready() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// my pieces of the stage have landed (N younger ones may be on their way) and my reads of the stage before are done; then
+// everybody's are
+template <int N> __device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+// everything has landed: nothing may be on its way into LDS when it is used for something else or the workgroup ends
+__device__ __forceinline__ void drain() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
 
-// acc[m][n] += sum over K steps k0 .. k1 of P[p0 + m][k] * Q[q0 + n][k]: both operands row by row along K
+// acc[m][n] += sum over K steps k0 .. k1 of P[p0 + m][k] * Q[q0 + n][k]: both operands row by row along K; the steps begin `turn`
+// further on and go round
 template <int F>
 __device__ __forceinline__ void product_rows(char* smem, const char* P, unsigned p_bytes, int p_rows, int p0, const char* Q, unsigned q_bytes,
-                                             int q_rows, int q0, int ld, int k0, int k1, float4_t (&acc)[F][F]) {
+                                             int q_rows, int q0, int ld, int k0, int k1, int turn, float4_t (&acc)[F][F]) {
     typedef Shape<F> S;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
@@ -213,13 +258,17 @@ __device__ __forceinline__ void product_rows(char* smem, const char* P, unsigned
         po[u] = p0 + row < p_rows ? (unsigned)(p0 + row) * (unsigned)(ld * 4) + chunk : BUF_OOB;
         qo[u] = q0 + row < q_rows ? (unsigned)(q0 + row) * (unsigned)(ld * 4) + chunk : BUF_OOB;
     }
+    // a step behind the last fetches nothing, but counts: the wait below is for a fixed number of loads
     auto issue = [&](int k, int buf) {
+        const bool live = k < k1;
+        k += turn;
+        if (k >= k1) k -= k1 - k0;
         const unsigned d = (unsigned)k * 128u;
 #pragma unroll
         for (int u = 0; u < S::PIECES / 4; ++u) {
             const unsigned dst = lds0 + buf * S::STAGE + (wave + 4 * u) * 1024;
-            glds16(rp, dst, po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
-            glds16(rq, dst + S::HALF, qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
+            glds16(rp, dst, !live || po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
+            glds16(rq, dst + S::HALF, !live || qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
         }
     };
     int pr[F], qr[F];
@@ -229,11 +278,13 @@ __device__ __forceinline__ void product_rows(char* smem, const char* P, unsigned
         pr[f] = m * 128 + ((lg ^ swz(m)) << 4);
         qr[f] = S::HALF + n * 128 + ((lg ^ swz(n)) << 4);
     }
-    if (k0 < k1) issue(k0, 0);
+    constexpr int AHEAD = S::STAGES - 1, LOADS = 2 * (S::PIECES / 4);      // loads of a wave and stage
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) issue(k0 + a, a);
     for (int k = k0; k < k1; ++k) {
-        const int buf = (k - k0) & 1;
-        stage_ready();
-        if (k + 1 < k1) issue(k + 1, buf ^ 1);
+        const int buf = (k - k0) % S::STAGES;
+        stage_ready<(AHEAD - 1) * LOADS>();
+        issue(k + AHEAD, (k - k0 + AHEAD) % S::STAGES);
         const char* s = smem + buf * S::STAGE;
         Frags<F> p, q;
 #pragma unroll
@@ -245,10 +296,12 @@ __device__ __forceinline__ void product_rows(char* smem, const char* P, unsigned
         }
         multiply<F>(p, q, acc);
     }
+    drain();
 }
 
 // acc[m][n] += sum over rows 32 k0 .. 32 k1 of X[r][p0 + m] * X[r][q0 + n]: K runs down the rows, so the fragments come through
-// the transposing LDS read.  A staged row holds T columns (hi and lo) = T * 4 bytes as 32-byte groups, XORed by the row.
+// the transposing LDS read.  A staged row holds T columns (hi and lo) = T * 4 bytes as 32-byte groups, XORed by the row.  On a
+// diagonal tile (p0 == q0) both operands are the same columns, staged once.
 template <int F>
 __device__ __forceinline__ void product_cols(char* smem, const char* X, unsigned bytes, int cols, int p0, int q0, int k0, int k1,
                                              float4_t (&acc)[F][F]) {
@@ -268,12 +321,13 @@ __device__ __forceinline__ void product_cols(char* smem, const char* X, unsigned
         qo[u] = q0 + byte / 4 < cols ? (unsigned)row * (unsigned)(cols * 4) + (unsigned)(q0 * 4 + byte) : BUF_OOB;
     }
     auto issue = [&](int k, int buf) {
+        const bool live = k < k1;
         const unsigned d = (unsigned)k * 32u * (unsigned)(cols * 4);
 #pragma unroll
         for (int u = 0; u < S::PIECES / 4; ++u) {
             const unsigned dst = lds0 + buf * S::STAGE + (wave + 4 * u) * 1024;
-            glds16(rs, dst, po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
-            glds16(rs, dst + S::HALF, qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
+            glds16(rs, dst, !live || po[u] == BUF_OOB ? BUF_OOB : po[u] + d);
+            if (p0 != q0) glds16(rs, dst + S::HALF, !live || qo[u] == BUF_OOB ? BUF_OOB : qo[u] + d);
         }
     };
     const int r1 = lg * 8 + (li >> 2);      // and r1 + 4, whose swizzle is the same
@@ -282,18 +336,21 @@ __device__ __forceinline__ void product_cols(char* smem, const char* X, unsigned
     for (int f = 0; f < F; ++f) {
         const int m = wm * F + f, n = wn * F + f;      // 16-column fragments: 32-byte group (m >> 1) * 4 + plane * 2 + (m & 1)
         pr[f] = lds0 + r1 * ROWB + ((((m >> 1) * 4 + (m & 1)) ^ tr_swz(r1)) * 32) + (li & 3) * 8;
-        qr[f] = lds0 + S::HALF + r1 * ROWB + ((((n >> 1) * 4 + (n & 1)) ^ tr_swz(r1)) * 32) + (li & 3) * 8;
+        qr[f] = lds0 + (p0 != q0 ? S::HALF : 0) + r1 * ROWB + ((((n >> 1) * 4 + (n & 1)) ^ tr_swz(r1)) * 32) + (li & 3) * 8;
     }
     auto tr2 = [&](unsigned a0) {
         const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(a0));
         const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(uintptr_t)(a0 + 4 * ROWB));
         return short8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     };
-    if (k0 < k1) issue(k0, 0);
+    constexpr int AHEAD = S::STAGES - 1, LOADS = S::PIECES / 4;      // of a wave, stage and operand
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) issue(k0 + a, a);
     for (int k = k0; k < k1; ++k) {
-        const int buf = (k - k0) & 1;
-        stage_ready();
-        if (k + 1 < k1) issue(k + 1, buf ^ 1);
+        const int buf = (k - k0) % S::STAGES;
+        if (p0 != q0) stage_ready<(AHEAD - 1) * 2 * LOADS>();
+        else stage_ready<(AHEAD - 1) * LOADS>();
+        issue(k + AHEAD, (k - k0 + AHEAD) % S::STAGES);
         const unsigned o = buf * S::STAGE;
         Frags<F> p, q;
 #pragma unroll
@@ -305,6 +362,7 @@ __device__ __forceinline__ void product_cols(char* smem, const char* X, unsigned
         }
         multiply<F>(p, q, acc);
     }
+    drain();
 }
 
 // lower-triangle tile `id` of a symmetric matrix: (row, col), col <= row
@@ -315,16 +373,20 @@ __device__ __forceinline__ void tri(int id, int& r, int& c) {
     c = id - r * (r + 1) / 2;
 }
 
-// The symmetric products A = X^T X (GRAM) and A A: the tiles on and below the diagonal, K cut into `splits` parts, f32
-// sums into slabs [split][tile][T][T].
+__device__ __forceinline__ float make_b(float a_old, float aa, bool diagonal) {
+    return fmaf(NS_B, a_old, NS_C * (aa * AB_FROM_AA)) + (diagonal ? NS_A * AB_SCALE : 0.f);
+}
+
+// The symmetric products A = X^T X (GRAM) and A A: the tiles on and below the diagonal.  Where K is cut (`splits` parts), f32 sums
+// into slabs [split][tile][T][T] for ns_fold_kernel; A A whole (splits 1) goes to B from here, both triangles.
 template <int F, bool GRAM>
 __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats ms, Starts st, Splits sp, int which, char* ws) {
     typedef Shape<F> S;
     __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
-    const int i = find(st, ms.n, blockIdx.x);
+    const int wg = xcd_id(), i = find(st, ms.n, wg);
     const Mat M = ms.m[i];
     const int nt = (M.Sp + S::T - 1) / S::T, tiles = nt * (nt + 1) / 2;
-    const int id = blockIdx.x - st.v[i], sl = id / tiles, t = id % tiles, splits = sp.v[i];
+    const int id = wg - st.v[i], sl = id / tiles, t = id % tiles, splits = sp.v[i];
     int r, c;
     tri(t, r, c);
     const int steps = (GRAM ? M.Lp : M.Sp) / 32, per = (steps + splits - 1) / splits;
@@ -338,11 +400,47 @@ __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats ms, Starts st, Spli
         product_cols<F>(smem, at(ws, which ? M.y1 : M.y0), (unsigned)((int64_t)M.Lp * M.Sp * 4), M.Sp, r * S::T, c * S::T, k0, k1, acc);
     } else {
         const unsigned bytes = (unsigned)((int64_t)M.Sp * M.Sp * 4);
-        product_rows<F>(smem, at(ws, M.a), bytes, M.Sp, r * S::T, at(ws, M.a), bytes, M.Sp, c * S::T, M.Sp, k0, k1, acc);
+        product_rows<F>(smem, at(ws, M.a), bytes, M.Sp, r * S::T, at(ws, M.a), bytes, M.Sp, c * S::T, M.Sp, k0, k1, 0, acc);
     }
     // [n][m]: a lane holds four consecutive m of one n
-    float* out = (float*)at(ws, M.slab) + ((int64_t)sl * tiles + t) * (S::T * S::T);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
+    if (!GRAM && splits == 1) {
+        const char* A = at(ws, M.a);
+        char* B = at(ws, M.b);
+#pragma unroll
+        for (int n = 0; n < F; ++n) {
+            __syncthreads();      // the stages (n = 0), the strip before
+            float* strip = reinterpret_cast<float*>(smem) + wave * 16 * (16 * F + 1);      // a wave's 16 rows (n) of 16 F columns (m)
+            const int gn = c * S::T + (wn * F + n) * 16;
+#pragma unroll
+            for (int m = 0; m < F; ++m) {
+                const int gm = r * S::T + (wm * F + m) * 16 + lg * 4;
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                if (gn < M.Sp && gm < M.Sp) {
+                    const char* q = A + cell(gn + li, M.Sp, gm);
+                    join4(*reinterpret_cast<const uint2*>(q), *reinterpret_cast<const uint2*>(q + 64), x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = make_b(x[e], acc[m][n][e], gn + li == gm + e);
+                    store4_split(B + cell(gn + li, M.Sp, gm), x);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) strip[li * (16 * F + 1) + m * 16 + lg * 4 + e] = x[e];
+            }
+            __syncthreads();
+            if (r == c) continue;      // a diagonal tile holds both triangles itself
+            // the mirror: rows gm .. of 16 columns gn ..
+            for (int i = lane; i < 16 * F * 4; i += 64) {
+                const int row = i >> 2, q4 = (i & 3) * 4, gm = r * S::T + wm * F * 16 + row;
+                if (gn >= M.Sp || gm >= M.Sp) continue;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = strip[(q4 + e) * (16 * F + 1) + row];
+                store4_split(B + cell(gm, M.Sp, gn + q4), x);
+            }
+        }
+        return;
+    }
+    float* out = (float*)at(ws, M.slab) + ((int64_t)sl * tiles + t) * (S::T * S::T);
 #pragma unroll
     for (int m = 0; m < F; ++m)
 #pragma unroll
@@ -350,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void ns_sym_kernel(Mats ms, Starts st, Spli
             *reinterpret_cast<float4_t*>(out + ((wn * F + n) * 16 + li) * S::T + (wm * F + m) * 16 + lg * 4) = acc[m][n];
 }
 
-// slabs -> A (GRAM) or B = b A + c A A, both triangles: a workgroup folds a 32 x 32 piece of a tile in slab order
+// slabs -> A (GRAM) or B, both triangles: a workgroup folds a 32 x 32 piece of a tile in slab order
 template <int F, bool GRAM>
 __global__ __launch_bounds__(256) void ns_fold_kernel(Mats ms, Starts st, Splits sp, char* ws) {
     typedef Shape<F> S;
@@ -358,6 +456,7 @@ __global__ __launch_bounds__(256) void ns_fold_kernel(Mats ms, Starts st, Splits
     const int i = find(st, ms.n, blockIdx.x);
     const Mat M = ms.m[i];
     const int nt = (M.Sp + S::T - 1) / S::T, tiles = nt * (nt + 1) / 2, splits = sp.v[i];
+    if (!GRAM && splits == 1) return;      // B is there
     const int id = blockIdx.x - st.v[i], t = id / (F * F), piece = id % (F * F);
     int r, c;
     tri(t, r, c);
@@ -369,7 +468,6 @@ __global__ __launch_bounds__(256) void ns_fold_kernel(Mats ms, Starts st, Splits
     float4_t v = *reinterpret_cast<const float4_t*>(src);
     for (int k = 1; k < splits; ++k) v += *reinterpret_cast<const float4_t*>(src + (int64_t)k * tiles * (S::T * S::T));
     float x[4];
-    uint2 hi, lo;
     if constexpr (GRAM) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = v[e] * AB_FROM_XX;
@@ -378,30 +476,26 @@ __global__ __launch_bounds__(256) void ns_fold_kernel(Mats ms, Starts st, Splits
         float old[4];
         join4(*reinterpret_cast<const uint2*>(a), *reinterpret_cast<const uint2*>(a + 64), old);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = fmaf(NS_B, old[e], NS_C * (v[e] * AB_FROM_AA));
+        for (int e = 0; e < 4; ++e) x[e] = make_b(old[e], v[e], gn + n == gm + m + e);
     }
     char* dst = at(ws, GRAM ? M.a : M.b);
-    split4(x, hi, lo);
-    char* q = dst + cell(gn + n, M.Sp, gm + m);
-    *reinterpret_cast<uint2*>(q) = hi;
-    *reinterpret_cast<uint2*>(q + 64) = lo;
+    store4_split(dst + cell(gn + n, M.Sp, gm + m), x);
     if (r == c) return;      // a diagonal tile holds both triangles itself
 #pragma unroll
     for (int e = 0; e < 4; ++e) tile[m + e][n] = x[e];
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = tile[n][m + e];
-    split4(x, hi, lo);
-    q = dst + cell(gm + n, M.Sp, gn + m);
-    *reinterpret_cast<uint2*>(q) = hi;
-    *reinterpret_cast<uint2*>(q + 64) = lo;
+    store4_split(dst + cell(gm + n, M.Sp, gn + m), x);
 }
 
-// X' = a X + X B.  The last step (LAST) writes the caller's matrix: X itself, or (MUON) the parameters.
+// X' = X B.  The last step (LAST) writes the caller's matrix: X itself, or (MUON) the parameters.
 template <int F, bool LAST, bool MUON>
 __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Starts st, Hyper h, int which, char* ws) {
     typedef Shape<F> S;
     __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
+    // block order as dispatched: an XCD's workgroups share one or two column tiles of B, which stay in its L2, and stream X (183 us
+    // at 2048 x 8192; with an XCD's blocks consecutive 205)
     const int i = find(st, ms.n, blockIdx.x);
     const Mat M = ms.m[i];
     const int nt = (M.Sp + S::T - 1) / S::T, id = blockIdx.x - st.v[i];
@@ -412,56 +506,187 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Star
     for (int m = 0; m < F; ++m)
 #pragma unroll
         for (int n = 0; n < F; ++n) acc[m][n] = float4_t{0.f, 0.f, 0.f, 0.f};
-    // rows of B (symmetric) against rows of X: a lane ends with four consecutive columns of one row of X
+    // Rows of B (symmetric) against rows of X: a lane ends with four consecutive columns of one row of X.  The K steps that hold
+    // this tile's part of B's diagonal, and with it a X, by far the largest term for a small singular value, come last: else every
+    // later addition rounds at its size (2048 x 8192: 4.0e-6 of the result instead of 1.7e-6)
+    const int steps = M.Sp / 32, turn = (s0 / 32 + S::T / 32) % steps;
     product_rows<F>(smem, at(ws, M.b), (unsigned)((int64_t)M.Sp * M.Sp * 4), M.Sp, s0, X, (unsigned)((int64_t)M.Lp * M.Sp * 4), M.Lp, l0,
-                    M.Sp, 0, M.Sp / 32, acc);
+                    M.Sp, 0, steps, turn, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, wm = wave >> 1, wn = wave & 1;
     const bool flip = M.rows < M.cols;
     bool skip = false;
     if constexpr (MUON) skip = skip_step(h);
+    const Io& io = ios.io[i];
+    // four columns of the caller's row at once where they lie so
+    const bool wide = LAST && !flip && (M.cols & 3) == 0 && ((reinterpret_cast<uintptr_t>(io.po) | (MUON ? reinterpret_cast<uintptr_t>(io.p) : 0)) & 15) == 0;
+    auto update = [&](float x, float p) { return skip ? p : p * (1.f - h.lr * h.wd) - h.lr * io.k * x; };
 #pragma unroll
     for (int n = 0; n < F; ++n) {
         const int l = l0 + (wn * F + n) * 16 + li;
-        if (l >= M.Lp) continue;
+        if (l >= (LAST ? (flip ? M.cols : M.rows) : M.Lp)) continue;
 #pragma unroll
         for (int m = 0; m < F; ++m) {
             const int s = s0 + (wm * F + m) * 16 + lg * 4;
-            if (s >= M.Sp) continue;
-            const int64_t o = cell(l, M.Sp, s);
+            if (s >= (LAST ? (flip ? M.rows : M.cols) : M.Sp)) continue;
             float x[4];
-            join4(*reinterpret_cast<const uint2*>(X + o), *reinterpret_cast<const uint2*>(X + o + 64), x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = fmaf(NS_A, x[e], acc[m][n][e] * X_FROM_XB);
+            for (int e = 0; e < 4; ++e) x[e] = acc[m][n][e] * (LAST ? X_FROM_XB * INV_X_SCALE : X_FROM_XB);
             if constexpr (!LAST) {
-                uint2 hi, lo;
-                split4(x, hi, lo);
-                char* q = at(ws, which ? M.y0 : M.y1) + o;
-                *reinterpret_cast<uint2*>(q) = hi;
-                *reinterpret_cast<uint2*>(q + 64) = lo;
+                store4_split(at(ws, which ? M.y0 : M.y1) + cell(l, M.Sp, s), x);
+            } else if (wide) {
+                const int64_t k = (int64_t)l * M.cols + s;
+                float4 o = make_float4(x[0], x[1], x[2], x[3]);
+                if constexpr (MUON) {
+                    const float4 p = *reinterpret_cast<const float4*>(io.p + k);
+                    o = make_float4(update(o.x, p.x), update(o.y, p.y), update(o.z, p.z), update(o.w, p.w));
+                }
+                *reinterpret_cast<float4*>(io.po + k) = o;
             } else {
-                const Io& io = ios.io[i];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int row = flip ? s + e : l, col = flip ? l : s + e;
-                    if (row >= M.rows || col >= M.cols) continue;
-                    const int64_t k = (int64_t)row * M.cols + col;
-                    const float v = x[e] * INV_X_SCALE;
-                    if constexpr (MUON) {
-                        const float p = io.p[k];
-                        io.po[k] = skip ? p : p * (1.f - h.lr * h.wd) - h.lr * io.k * v;
-                    } else {
-                        io.po[k] = v;
-                    }
+                    if (s + e >= (flip ? M.rows : M.cols)) continue;
+                    const int64_t k = flip ? (int64_t)(s + e) * M.cols + l : (int64_t)l * M.cols + s + e;
+                    io.po[k] = MUON ? update(x[e], io.p[k]) : x[e];
                 }
             }
         }
     }
 }
 
+// ------------------------------------------------------------------------------------------------------------------- small
+// A matrix with S <= SMALL_S and L <= SMALL_L: one workgroup does everything, X, A and B as f32 in LDS, the products on the f32
+// matrix cores (16 x 16 x 4; they have a sixteenth of the f16 rate, but the launches of the general form alone take longer).  Five
+// steps: 16 x 16 9 us, 64 x 18 19, 128 x 64 59, 256 x 64 102; the general form takes 82 at 257 x 64.
+constexpr int SMALL_S = 64, SMALL_L = 192, SMALL_THREADS = 512, SMALL_WAVES = SMALL_THREADS / 64;
+inline bool is_small(int r, int c) { return (r > c ? c : r) <= SMALL_S && (r > c ? r : c) <= SMALL_L; }
+__host__ __device__ inline int up16(int v) { return (v + 15) & ~15; }
+inline size_t small_lds(int r, int c) {
+    const int L = up16(r > c ? r : c), S = up16(r > c ? c : r), ld = S + 4;
+    return ((size_t)L + 2 * S) * ld * sizeof(float);
+}
+struct Smalls { int rows[CUTIE_MAX_BATCH], cols[CUTIE_MAX_BATCH]; };
+
+// acc[c] += P(row m, k) Q(k, column n) over k = 0 .. K-1 for NC column blocks: pa = P's address of (m = li, k = lg), pk its
+// step per k; qa = Q's address of (k = lg, n = li), qk likewise
+template <int NC>
+__device__ __forceinline__ void small_product(const float* pa, int pk, const float* qa, int qk, int K, int nc, float4_t (&acc)[NC]) {
+    for (int k = 0; k < K; k += 16) {      // K is a multiple of 16; four steps' operands are on their way together
+        float a[4], q[4][NC];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = pa[(k + j * 4) * pk];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) q[j][c] = c < nc ? qa[(k + j * 4) * qk + c * 16] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (c < nc) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], q[j][c], acc[c], 0, 0, 0);
+    }
+}
+
+template <bool MUON>
+__global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios ios, Hyper h, int steps, float eps) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    __shared__ double part[SMALL_WAVES];
+    const int rows = sm.rows[blockIdx.x], cols = sm.cols[blockIdx.x];
+    const Io io = ios.io[blockIdx.x];
+    const bool flip = rows < cols;
+    const int L = up16(flip ? cols : rows), S = up16(flip ? rows : cols), ld = S + 4;      // + 4: the 16 rows of a fragment on 64 banks
+    float* X = lds;                // [L][ld]
+    float* A = X + L * ld;         // [S][ld]
+    float* B = A + S * ld;         // [S][ld]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    const bool skip = MUON && skip_step(h);
+    float inv = 1.f, scale = 1.f;
+    if constexpr (MUON) {
+        inv = h.loss_scale ? h.loss_scale[1] : 1.f;
+        scale = clip_scale(h);
+    }
+    for (int i = threadIdx.x; i < L * ld; i += SMALL_THREADS) X[i] = 0.f;
+    __syncthreads();
+    double sum = 0;
+    for (int i = threadIdx.x; i < rows * cols; i += SMALL_THREADS) {
+        const int r = i / cols, c = i - r * cols;
+        float v;
+        if constexpr (MUON) {
+            const float g = (io.g[i] * inv + h.l2 * io.p[i]) * scale, m0 = io.m[i], m1 = h.mu * m0 + g;
+            v = h.nesterov ? g + h.mu * m1 : m1;
+            io.mo[i] = skip ? m0 : m1;
+        } else {
+            v = io.g[i];
+        }
+        X[flip ? c * ld + r : r * ld + c] = v;
+        sum = fma((double)v, (double)v, sum);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    sum = part[0];
+    for (int w = 1; w < SMALL_WAVES; ++w) sum += part[w];
+    const float k = (float)(1.0 / (sqrt(sum) + (double)eps));
+    for (int i = threadIdx.x; i < L * ld; i += SMALL_THREADS) X[i] *= k;
+    __syncthreads();
+    const int sb = S / 16, lb = L / 16;
+    for (int step = 0; step < steps; ++step) {
+        // A = X^T X, 16 x 16 blocks round the waves; a lane ends with rows lg * 4 .. of one column
+        for (int t = wave; t < sb * sb; t += SMALL_WAVES) {
+            const int m0 = t / sb * 16, n0 = t % sb * 16;
+            float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
+            small_product<1>(X + lg * ld + m0 + li, ld, X + lg * ld + n0 + li, ld, L, 1, acc);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) A[(m0 + lg * 4 + e) * ld + n0 + li] = acc[0][e];
+        }
+        __syncthreads();
+        // B = a I + b A + c A A
+        for (int t = wave; t < sb * sb; t += SMALL_WAVES) {
+            const int m0 = t / sb * 16, n0 = t % sb * 16;
+            float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
+            small_product<1>(A + (m0 + li) * ld + lg, 1, A + lg * ld + n0 + li, ld, S, 1, acc);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int m = m0 + lg * 4 + e, n = n0 + li;
+                B[m * ld + n] = fmaf(NS_B, A[m * ld + n], NS_C * acc[0][e]) + (m == n ? NS_A : 0.f);
+            }
+        }
+        __syncthreads();
+        // X = X B: a wave's 16 rows depend on themselves alone
+        for (int t = wave; t < lb; t += SMALL_WAVES) {
+            float4_t acc[SMALL_S / 16];
+#pragma unroll
+            for (int c = 0; c < SMALL_S / 16; ++c) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+            small_product<SMALL_S / 16>(X + (t * 16 + li) * ld + lg, 1, B + lg * ld + li, ld, S, sb, acc);
+#pragma unroll
+            for (int c = 0; c < SMALL_S / 16; ++c)
+                if (c < sb) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) X[(t * 16 + lg * 4 + e) * ld + c * 16 + li] = acc[c][e];
+                }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < rows * cols; i += SMALL_THREADS) {
+        const int r = i / cols, c = i - r * cols;
+        const float v = X[flip ? c * ld + r : r * ld + c];
+        if constexpr (MUON) {
+            const float p = io.p[i];
+            io.po[i] = skip ? p : p * (1.f - h.lr * h.wd) - h.lr * io.k * v;
+        } else {
+            io.po[i] = v;
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------- host
 struct NsPlan {
-    Mats ms;
+    Mats ms;                 // the matrices of the general form
+    Smalls sm;               // those of the small one
+    int n_small, order[CUTIE_MAX_BATCH];      // the caller's index of each: the general ones, then the small ones
+    size_t lds;              // of the small form
     Splits gram, square;
+    bool fold_square;        // some A A is cut along K
     int fg, fs, fa;          // tile factors (4: 128 x 128, 2: 64 x 64) of the three products
     size_t bytes;
 };
@@ -471,18 +696,33 @@ inline int tri_tiles(int Sp, int f) { const int nt = (int)cdiv(Sp, 32 * f); retu
 // shapes: (rows, cols) of n matrices
 inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
     CUTIE_CHECK_ARG(n >= 1 && n <= CUTIE_MAX_BATCH, "%s: %d matrices (1..%d)", who, n, CUTIE_MAX_BATCH);
-    p.ms.n = n;
+    p.ms.n = p.n_small = 0;
+    p.fold_square = false;
+    p.lds = 0;
     for (int i = 0; i < n; ++i) {
         const int r = shapes[2 * i], c = shapes[2 * i + 1];
         CUTIE_CHECK_ARG(r >= 1 && c >= 1, "%s: matrix %d is %d x %d", who, i, r, c);
+        if (is_small(r, c)) continue;
         const int64_t Lp = cdiv(r > c ? r : c, 64) * 64, Sp = cdiv(r > c ? c : r, 64) * 64;
         CUTIE_CHECK_ARG(Lp * Sp < ((int64_t)1 << 29), "%s: matrix %d is %d x %d (padded to multiples of 64, below 2^29 values)", who, i, r, c);
-        p.ms.m[i].rows = r;
-        p.ms.m[i].cols = c;
-        p.ms.m[i].Lp = (int)Lp;
-        p.ms.m[i].Sp = (int)Sp;
+        Mat& m = p.ms.m[p.ms.n];
+        m.rows = r;
+        m.cols = c;
+        m.Lp = (int)Lp;
+        m.Sp = (int)Sp;
+        p.order[p.ms.n++] = i;
     }
-    // the 128 tile where it alone gives the chip two workgroups a CU or (with K cut) K is long enough to be cut
+    for (int i = 0; i < n; ++i) {
+        const int r = shapes[2 * i], c = shapes[2 * i + 1];
+        if (!is_small(r, c)) continue;
+        p.sm.rows[p.n_small] = r;
+        p.sm.cols[p.n_small] = c;
+        p.order[p.ms.n + p.n_small++] = i;
+        if (small_lds(r, c) > p.lds) p.lds = small_lds(r, c);
+    }
+    n = p.ms.n;
+    // The 128 tile where it gives every CU a workgroup, K cut into pieces of eight steps where it can be (14 filters: 475 us; with
+    // the 64 tile for X B 526, for X^T X 532); two workgroups a CU by cutting K (512 / tiles: 475 us, 256 530, 1024 538)
     int64_t tg = 0, ts = 0, ta = 0;
     for (int i = 0; i < n; ++i) {
         const Mat& m = p.ms.m[i];
@@ -494,6 +734,7 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
     p.fs = ts >= 256 ? 4 : 2;
     p.fa = ta >= 256 ? 4 : 2;
     int64_t ng = 0, nq = 0;
+    if (!n) { p.bytes = 256; return CUTIE_OK; }      // no workspace needed; a size all the same
     for (int i = 0; i < n; ++i) { ng += tri_tiles(p.ms.m[i].Sp, p.fg); nq += tri_tiles(p.ms.m[i].Sp, p.fs); }
     size_t off = 0;
     auto take = [&](int64_t bytes) {
@@ -508,7 +749,9 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
             return (short)(s < 1 ? 1 : (s > 64 ? 64 : s));
         };
         p.gram.v[i] = cut(512 / ng, m.Lp / 32);
-        p.square.v[i] = cut(512 / nq, m.Sp / 32);
+        // A A is cut only where K is long: at S = 256 its eight steps take less than a fold of the parts
+        p.square.v[i] = m.Sp > 512 ? cut(512 / nq, m.Sp / 32) : (short)1;
+        if (p.square.v[i] > 1) p.fold_square = true;
         const int64_t y = (int64_t)m.Lp * m.Sp * 4, a = (int64_t)m.Sp * m.Sp * 4;
         const int64_t sg = (int64_t)p.gram.v[i] * tri_tiles(m.Sp, p.fg) * (32 * p.fg) * (32 * p.fg) * 4;
         const int64_t ss = (int64_t)p.square.v[i] * tri_tiles(m.Sp, p.fs) * (32 * p.fs) * (32 * p.fs) * 4;
@@ -539,6 +782,7 @@ template <int F, bool GRAM> inline void ns_sym(const NsPlan& p, int which, char*
     Starts st;
     const unsigned g = starts(p, st, [&](const Mat& m, int i) { return (int64_t)tri_tiles(m.Sp, F) * sp.v[i]; });
     hipLaunchKernelGGL((ns_sym_kernel<F, GRAM>), dim3(g), dim3(256), 0, stream, p.ms, st, sp, which, ws);
+    if (!GRAM && !p.fold_square) return;
     const unsigned f = starts(p, st, [&](const Mat& m, int) { return (int64_t)tri_tiles(m.Sp, F) * F * F; });
     hipLaunchKernelGGL((ns_fold_kernel<F, GRAM>), dim3(f), dim3(256), 0, stream, p.ms, st, sp, ws);
 }
@@ -551,8 +795,18 @@ inline void ns_apply(const NsPlan& p, const Ios& ios, const Hyper& h, int which,
     else hipLaunchKernelGGL((ns_apply_kernel<F, false, false>), dim3(g), dim3(256), 0, stream, p.ms, ios, st, h, which, ws);
 }
 
-template <bool MUON> inline int ns_run(const NsPlan& p, const Ios& ios, const Hyper& h, int steps, float eps, char* ws, hipStream_t stream) {
+template <bool MUON>
+inline int ns_run(const NsPlan& p, const Ios& given, const Hyper& h, int steps, float eps, char* ws, hipStream_t stream) {
     static_assert(sizeof(Mats) + sizeof(Ios) + sizeof(Starts) + sizeof(Hyper) + 64 < 4096, "kernel arguments");
+    Ios ios = {};
+    if (p.n_small) {
+        for (int i = 0; i < p.n_small; ++i) ios.io[i] = given.io[p.order[p.ms.n + i]];
+        CUTIE_ENSURE_LDS(ns_small_kernel<MUON>, p.lds);
+        hipLaunchKernelGGL((ns_small_kernel<MUON>), dim3((unsigned)p.n_small), dim3(SMALL_THREADS), p.lds, stream, p.sm, ios, h, steps, eps);
+        CUTIE_CHECK_LAUNCH();
+    }
+    if (!p.ms.n) return CUTIE_OK;
+    for (int i = 0; i < p.ms.n; ++i) ios.io[i] = given.io[p.order[i]];
     Starts st;
     const unsigned g0 = starts(p, st, [](const Mat& m, int) { return cdiv((int64_t)m.rows * m.cols, NORM_CHUNK); });
     hipLaunchKernelGGL((ns_norm_kernel<MUON>), dim3(g0), dim3(256), 0, stream, p.ms, ios, st, h, ws);

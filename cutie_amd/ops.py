@@ -665,10 +665,6 @@ def _matrix(t, what, like=None):
     return t.numel() // t.shape[-1], t.shape[-1]
 
 
-def _overlap(a, b):
-    return a.data_ptr() < b.data_ptr() + b.numel() * 4 and b.data_ptr() < a.data_ptr() + a.numel() * 4
-
-
 def orthogonalize_workspace_bytes(shapes):
     """shapes: (rows, cols) of each matrix of one call, in order"""
     flat = (ctypes.c_int * (2 * max(1, len(shapes))))(*[int(v) for s in shapes for v in s])
@@ -710,20 +706,25 @@ def muon_descs(entries):
         raise capi.CutieError("muon_step: %d matrices (1..%d)" % (len(entries), capi.MAX_BATCH))
     arr = (capi.MuonDesc * len(entries))()
     shapes = []
+    device = entries[0][0].device
     for i, (p, g, m, p_out, m_out, out_scale) in enumerate(entries):
-        shapes.append(_matrix(p, "muon_step"))
+        rows, cols = _matrix(p, "muon_step")
         for t in (g, m, p_out, m_out):
-            _matrix(t, "muon_step", p)
-        if p.device != entries[0][0].device:
+            if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous() or t.device != device:
+                _matrix(t, "muon_step", p)
+        if p.device != device:
             raise capi.CutieError("muon_step: matrices on different devices")
-        if any(_overlap(a, b) for a, b in ((p_out, g), (p_out, m), (p_out, m_out), (m_out, g), (m_out, p))):
+        pp, pg, pm, qp, qm = ptr(p), ptr(g), ptr(m), ptr(p_out), ptr(m_out)
+        n = rows * cols * 4
+        # an output may be its own input, and overlaps nothing else
+        if (abs(qp - qm) < n or abs(qp - pg) < n or abs(qp - pm) < n or abs(qm - pg) < n or abs(qm - pp) < n
+                or 0 < abs(qp - pp) < n or 0 < abs(qm - pm) < n):
             raise capi.CutieError("muon_step: matrix %d: an output overlaps another tensor" % i)
-        if any(_overlap(a, b) and a.data_ptr() != b.data_ptr() for a, b in ((p_out, p), (m_out, m))):
-            raise capi.CutieError("muon_step: matrix %d: an output may be its input, not overlap a part of it" % i)
         d = arr[i]
-        d.p, d.g, d.m, d.p_out, d.m_out = ptr(p), ptr(g), ptr(m), ptr(p_out), ptr(m_out)
-        d.rows, d.cols, d.out_scale = shapes[-1][0], shapes[-1][1], float(out_scale)
-    return arr, shapes, entries[0][0].device
+        d.p, d.g, d.m, d.p_out, d.m_out = pp, pg, pm, qp, qm
+        d.rows, d.cols, d.out_scale = rows, cols, out_scale
+        shapes.append((rows, cols))
+    return arr, shapes, device
 
 
 def muon_step(entries, lr, momentum=0.95, nesterov=True, weight_decay=0.0, l2=0.0, steps=5, eps=ORTH_EPS, gnorm_sq=None, clip=0.0,

@@ -88,7 +88,8 @@ def matrix(r, c, kind, g):
 
 
 SIZES = [(1, 1), (1, 7), (9, 1), (2, 2), (18, 64), (64, 18), (63, 65), (64, 64), (65, 129), (128, 128), (300, 129), (256, 1000),
-         (1920, 256), (130, 4000), (700, 700)]
+         (1920, 256), (130, 4000), (700, 700),
+         (192, 64), (64, 192), (193, 64), (64, 193), (192, 65), (3000, 20), (520, 530)]      # both sides of the one-workgroup form
 
 
 @pytest.mark.gpu
@@ -131,7 +132,7 @@ def test_steps(steps):
 @pytest.mark.gpu
 def test_batch_of_every_shape():
     g = torch.Generator().manual_seed(5)
-    shapes = (SIZES * 3)[:32]
+    shapes = (SIZES * 2)[:32]
     us = [matrix(r, c, ("normal", "falling")[i % 2], g) * 10.0 ** (i % 7 - 3) for i, (r, c) in enumerate(shapes)]
     ds = [u.to(DEV) for u in us]
     outs = [torch.full_like(d, 7.0) for d in ds]
@@ -318,7 +319,7 @@ def orth_rc(rows=4, cols=3, n=1, steps=5, eps=1e-7, g=P(4096), out=P(8192), ws=P
     (dict(rows=0), -1, b"0 x 3"), (dict(cols=-1), -1, b"4 x -1"), (dict(n=0), -1, b"0 matrices"), (dict(n=33), -1, b"33 matrices"),
     (dict(steps=0), -1, b"steps"), (dict(steps=33), -1, b"steps"), (dict(eps=0.0), -1, b"eps"), (dict(g=None), -1, b"null"),
     (dict(out=P(8193)), -1, b"misaligned"), (dict(rows=1 << 20, cols=1 << 10), -1, b"2^29"), (dict(ws=None), -3, b"workspace"),
-    (dict(nbytes=256), -3, b"workspace"), (dict(ws=P((1 << 20) + 16)), -3, b"workspace")])
+    (dict(nbytes=255), -3, b"workspace"), (dict(ws=P((1 << 20) + 16)), -3, b"workspace"), (dict(rows=300, cols=200, nbytes=4096), -3, b"workspace")])
 def test_orthogonalize_refusals(kw, rc, word):
     assert orth_rc(**kw) == rc and word in capi.lib().cutie_last_error()
 
@@ -340,7 +341,8 @@ def test_muon_refusals():
 
 
 def test_workspace_bytes():
-    assert ops.orthogonalize_workspace_bytes([(64, 18)]) >= 2 * 64 * 64 * 4
+    assert ops.orthogonalize_workspace_bytes([(64, 18)]) > 0
+    assert ops.orthogonalize_workspace_bytes([(64, 18), (300, 200)]) >= 2 * 320 * 256 * 4
     assert ops.orthogonalize_workspace_bytes([(0, 18)]) == 0 and ops.orthogonalize_workspace_bytes([(4, 4)] * 33) == 0
 
 
@@ -356,3 +358,15 @@ def test_wrapper_refusals():
                 lambda: ops.muon_descs([(big[:24].view(4, 6), w.clone(), w.clone(), big[6:30].view(4, 6), w, 1.0)])):
         with pytest.raises(capi.CutieError):
             bad()
+
+
+@pytest.mark.gpu
+def test_overlapping_outputs_are_refused():
+    w = torch.zeros(400, device=DEV)
+    g, m = torch.zeros(4, 6, device=DEV), torch.zeros(4, 6, device=DEV)
+    p = w[:24].view(4, 6)
+    for po, mo in ((w[6:30].view(4, 6), m), (g, m), (m, m), (p, p), (p, g), (p, w[12:36].view(4, 6))):
+        with pytest.raises(capi.CutieError, match="overlaps"):
+            ops.muon_descs([(p, g, m, po, mo, 1.0)])
+    ops.muon_descs([(p, g, m, p, m, 1.0)])
+    ops.muon_descs([(p, g, m, w[24:48].view(4, 6), m, 1.0)])
