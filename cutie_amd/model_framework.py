@@ -95,12 +95,14 @@ class Model(object):
 
     # ------------------------------------------------------------------ hot-path ops
     @layer
-    def embed(self, layer_input, vocabulary_size, embedding_size, name, dropout=1, trainable=True):
+    def embed(self, layer_input, vocabulary_size, embedding_size, name, dropout=1, trainable=True, scale=1.0):
+        """scale (no counterpart in the reference): the looked-up rows are multiplied by it; its gradient is taken by sorted
+        tokens (cutie_embed_grad_sorted)."""
         if dropout != 1:
             # data_augmentation_dropout is a keep-prob that the reference leaves at 1 (identity)
             raise NotImplementedError("embedding dropout keep_prob %r != 1 is not built" % (dropout,))
         self.make_var(name + "/weights", [vocabulary_size, embedding_size], "uniform(-1,1)", None, trainable)
-        return Node(name, "embed", [layer_input], {"V": vocabulary_size, "E": embedding_size},
+        return Node(name, "embed", [layer_input], {"V": vocabulary_size, "E": embedding_size, "scale": float(scale)},
                     channels=embedding_size, domain="grid")
 
     @layer
@@ -109,14 +111,30 @@ class Model(object):
         return Node(name, "positional_sampling", [featuremap, batch_indices, grid], {},
                     channels=feature_dimension, domain="grid")
 
-    def _conv_node(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable):
+    def _conv_node(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable, norm="instance", groups=32):
+        """norm "instance" (the reference's): instance_norm(act(conv + bias)).  norm "group" (no counterpart there): act(group
+        norm(conv)) with `groups` groups of channels, '<name>/gamma' and '<name>/beta' in place of the bias, and 'silu' or
+        'none' as activations too (cutie_gn_fwd)."""
         if (s_h, s_w) != (1, 1):
             raise NotImplementedError("strided convolution is outside the hot-path scope (stride %r)" % ((s_h, s_w),))
-        if activation not in ("relu", "sigmoid"):
-            activation = "relu"    # model_framework.py:173-175: anything but 'sigmoid' is relu
+        if norm not in ("instance", "group"):
+            raise ValueError("norm %r (instance, group)" % (norm,))
         if isinstance(layer_input, list):
             raise ValueError("conv takes one input, got %d" % len(layer_input))
         c_i = layer_input.channels
+        if norm == "group":
+            if activation not in ("relu", "sigmoid", "silu", "none"):
+                raise ValueError("activation %r of a group-normalised layer (relu, sigmoid, silu, none)" % (activation,))
+            if groups < 1 or c_o % groups:
+                raise ValueError("%d groups do not divide %d channels" % (groups, c_o))
+            self.make_var(name + "/weights", [k_h, k_w, c_i, c_o], "truncated_normal(0,0.01)", True, trainable)
+            self.make_var(name + "/gamma", [c_o], "ones", None, trainable)
+            self.make_var(name + "/beta", [c_o], "zeros", None, trainable)
+            return Node(name, "conv", [layer_input],
+                        {"kh": k_h, "kw": k_w, "rate": rate, "activation": activation, "cin": c_i, "norm": "group",
+                         "groups": int(groups)}, channels=c_o, domain=layer_input.domain)
+        if activation not in ("relu", "sigmoid"):
+            activation = "relu"    # model_framework.py:173-175: anything but 'sigmoid' is relu
         self.convolution(None, activation, layer_input, k_h, k_w, c_i, c_o, "truncated_normal(0,0.01)", "zeros",
                          True, trainable, scope=name)
         return Node(name, "conv", [layer_input],
@@ -124,16 +142,16 @@ class Model(object):
                     channels=c_o, domain=layer_input.domain)
 
     @layer
-    def conv(self, layer_input, k_h, k_w, c_o, s_h, s_w, name, activation="relu", trainable=True):
-        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, 1, name, activation, trainable)
+    def conv(self, layer_input, k_h, k_w, c_o, s_h, s_w, name, activation="relu", trainable=True, norm="instance", groups=32):
+        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, 1, name, activation, trainable, norm, groups)
 
     @layer
-    def dilate_conv(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation="relu", trainable=True):
-        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable)
+    def dilate_conv(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation="relu", trainable=True, norm="instance", groups=32):
+        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable, norm, groups)
 
     @layer
-    def dilate_module(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation="relu", trainable=True):
-        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable)
+    def dilate_module(self, layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation="relu", trainable=True, norm="instance", groups=32):
+        return self._conv_node(layer_input, k_h, k_w, c_o, s_h, s_w, rate, name, activation, trainable, norm, groups)
 
     @layer
     def concat(self, layer_input, axis, name):

@@ -32,16 +32,29 @@ def _pad(c, m=64):
     return (c + m - 1) // m * m
 
 
+def _group(node):
+    """whether a conv node ends in a group norm (its variables are weights, gamma and beta)"""
+    return node.attrs.get("norm") == "group"
+
+
+def _scale(node):
+    """factor of an embedding's looked-up rows"""
+    return node.attrs.get("scale", 1.0)
+
+
 class _Plan(object):
     pass
 
 
 class Engine(object):
-    def __init__(self, network, device="cuda:0", dtype="f16", seed=0, loss_scale=None, overlap_wgrad=None, max_plans=4):
+    def __init__(self, network, device="cuda:0", dtype="f16", seed=0, loss_scale=None, overlap_wgrad=None, max_plans=4,
+                 embed_grad="atomic"):
         """dtype: 'f16' (the headline path: IEEE half activations and MFMA operands, f32 accumulation, statistics
         and parameters; meets the 2e-2 logit tolerance; backward runs under a dynamic loss scale kept on the device,
         initial value `loss_scale`, default 4096), 'bf16' (same tiles and MFMA rate, 8 significant bits: outside the
-        tolerance on deep stacks, kept as an option) or 'f32' (parity mode, 1e-4)."""
+        tolerance on deep stacks, kept as an option) or 'f32' (parity mode, 1e-4).
+        embed_grad: 'atomic' (cutie_embed_bwd: float atomics for ids >= 2) or 'sorted' (cutie_embed_grad_sorted: the same bits
+        every run; always taken by an embedding with a scale)."""
         capi.lib()   # fail loudly, before anything else, when the HIP library is absent
         if not torch.cuda.is_available():
             raise CutieError("cutie_amd needs a HIP device (torch.cuda.is_available() is False); there is no CPU path")
@@ -68,6 +81,12 @@ class Engine(object):
         self.overlap_wgrad = bool(overlap_wgrad)
         self._side = None
         self.C = network.num_classes
+        if embed_grad not in ("atomic", "sorted"):
+            raise CutieError("embed_grad %r (atomic, sorted)" % (embed_grad,))
+        self.embed_sorted = embed_grad == "sorted"
+        logits = network.layers.get(getattr(network, "loss_logits_name", None))
+        if logits is not None and _group(logits):
+            raise NotImplementedError("the loss head needs its logits layer instance-normalised")
         # buffer sets per (B, H, W, Hi), least recently used first.  The reference's loader draws a new grid shape for
         # almost every training batch (data_loader_json.py:660-694: max over the documents plus |N(0,16)| padding), and
         # one set is ~4 GB at B = 32, 64 x 64: only the `max_plans` most recently used shapes keep theirs.
@@ -125,7 +144,7 @@ class Engine(object):
             elif len(s.shape) == 4:
                 p = torch.nn.init.trunc_normal_(torch.empty(s.shape), mean=0.0, std=0.01, a=-0.02, b=0.02, generator=g)
             else:
-                p = torch.zeros(s.shape)
+                p = torch.ones(s.shape) if s.init == "ones" else torch.zeros(s.shape)      # a group norm's gamma
             self.params[s.name].copy_(p)
         self.repack()
 
@@ -213,6 +232,8 @@ class Engine(object):
         n_stats = sum(B * tiles[n.name] * n.channels * 2 for n in convs)
         P.stats_all = torch.zeros(n_stats, dtype=torch.float32, device=dev)
         P.a, P.stats, P.red, P.dz, P.dy, P.dbpart, P.sync, P.sync_fw, P.fused = {}, {}, {}, {}, {}, {}, {}, {}, {}
+        P.gn_stats = {}      # (mean, 1/sigma) of the group-normalised layers
+        gn_ws = 0
         so = 0
         for n in convs:
             hs, ws = spatial(n)
@@ -220,6 +241,10 @@ class Engine(object):
             cnt = B * tiles[n.name] * n.channels * 2
             P.stats[n.name] = P.stats_all[so:so + cnt].view(B, tiles[n.name], n.channels, 2)
             so += cnt
+            if _group(n):
+                P.gn_stats[n.name] = torch.zeros((B, n.attrs["groups"], 2), dtype=torch.float32, device=dev)
+                gn_ws = max(gn_ws, ops.gn_workspace_bytes(B, hs * ws, n.channels, n.attrs["groups"]))
+        P.gn_ws = torch.empty(max(gn_ws, 16), dtype=torch.uint8, device=dev)
         pooled = [n.inputs[0].channels for n in nodes if n.op == "global_pool"]
         P.pool_scratch = (torch.zeros(B * capi.POOL_TILES * max(pooled) * 2, dtype=torch.float32, device=dev)
                           if pooled else None)
@@ -360,7 +385,7 @@ class Engine(object):
                 self._walk_consumers(P, c.name, off + o, segs)
             elif c.op == "global_pool":
                 # dropping this gradient is exact only behind an instance norm ('global pool gradient')
-                if self.net.layers[nm].op != "conv":
+                if self.net.layers[nm].op != "conv" or _group(self.net.layers[nm]):
                     raise NotImplementedError("gradient of global_pool(%s): the pooled tensor is not the output of an "
                                               "instance-normalised conv, so the pool's gradient does not vanish" % nm)
             elif c.op in ("softmax", "positional_sampling"):
@@ -386,6 +411,8 @@ class Engine(object):
         backward pass uses).  From a where it was stored; where only y was, from y's encoding: the a == 0 elements of a
         (sample, channel) plane all hold the plane's smallest value y0 = round16((0 - mean) * inv)."""
         n = self.net.layers[name]
+        if _group(n):
+            raise CutieError("%s is group-normalised: its activation follows the norm" % name)
         if n is P.head:
             return P.head_a[..., :n.channels] > 0
         if not P.fused.get(name):
@@ -427,7 +454,7 @@ class Engine(object):
             ops.batch_scatter_add(dps.as_strided((P.B, P.H * P.W, C), (dps.stride(0), dps.stride(2), 1)), P.ps, acc)
             ops.convert(acc.view(P.B, P.Hi, P.W, C), P.dy[n.name][..., :C])
         elif segs:
-            if n.op == "conv":
+            if n.op == "conv" and not _group(n):
                 av, from_y = self._act_operand(P, n)
                 ops.conv_dgrad_in_bwd(segs, P.dy[n.name][..., :n.channels], n.channels, av,
                                       P.stats[n.name], P.red[n.name], P.dz[n.name][..., :n.channels],
@@ -480,7 +507,10 @@ class Engine(object):
         P.counters.zero_()
         for n in net.nodes:
             if n.op == "embed":
-                ops.embed_fwd(P.grid, self.params[n.name + "/weights"], P.view(n.name, n.channels), P.oob)
+                if _scale(n) == 1.0:
+                    ops.embed_fwd(P.grid, self.params[n.name + "/weights"], P.view(n.name, n.channels), P.oob)
+                else:
+                    ops.embed_scaled_fwd(P.grid, self.params[n.name + "/weights"], P.view(n.name, n.channels), _scale(n), P.oob)
             elif n.op == "conv" and n is P.head:
                 # the logits layer, its norm, the softmax and (training) the CE + level 0 of the hard-negative select
                 a = n.attrs
@@ -499,6 +529,14 @@ class Engine(object):
                 cin_pad = _pad(a["cin"], self.bke)
                 seg = [dict(x=P.view(src.name, cin_pad), w=self.w_fwd[n.name + "/weights"], cin=cin_pad,
                             kh=a["kh"], kw=a["kw"], dil=a["rate"])]
+                if _group(n):
+                    # act(group norm(conv)): no bias (beta follows the norm)
+                    P.fused[n.name] = False
+                    ops.conv_fwd(seg, P.a[n.name], n.channels)
+                    ops.gn_fwd(P.a[n.name][..., :n.channels], P.view(n.name, n.channels), P.gn_stats[n.name],
+                               gamma=self.params[n.name + "/gamma"], beta=self.params[n.name + "/beta"], act=a["activation"],
+                               workspace=P.gn_ws)
+                    continue
                 bias, act = self.params[n.name + "/biases"], a.get("activation", "relu")
                 if self.dt != F32 and P.view(n.name, n.channels).dtype == self.tdt and (
                         labels is None or (act != "sigmoid" and self.train_fwd_fused)):
@@ -676,7 +714,12 @@ class Engine(object):
             if n.op == "conv":
                 a = n.attrs
                 have_dz = self._backprop_into(P, n) if n.name != lname else (n is P.head)
-                if not have_dz:
+                if _group(n):
+                    ops.gn_bwd(P.dy[n.name][..., :n.channels], P.a[n.name][..., :n.channels], P.gn_stats[n.name],
+                               P.dz[n.name][..., :n.channels], gamma=self.params[n.name + "/gamma"],
+                               beta=self.params[n.name + "/beta"], act=a["activation"], dgamma=self.grads[n.name + "/gamma"],
+                               dbeta=self.grads[n.name + "/beta"], workspace=P.gn_ws)
+                elif not have_dz:
                     dy = P.dy[n.name][..., :n.channels]
                     av, from_y = self._act_operand(P, n)
                     bias, act = self.params[n.name + "/biases"], a.get("activation", "relu")
@@ -709,11 +752,18 @@ class Engine(object):
                 self._backprop_into(P, n)
             elif n.op == "embed":
                 self._backprop_into(P, n)
+                by_sort = self.embed_sorted or _scale(n) != 1.0
                 if getattr(P, "embed_ws", None) is None:
-                    P.embed_ws = torch.empty(ops.embed_bwd_workspace_bytes(P.grid.numel(), n.channels), dtype=torch.uint8,
-                                             device=self.dev)
-                ops.embed_bwd(P.grid, P.dy[n.name][..., :n.channels], self.grads[n.name + "/weights"], P.embed_ws)
+                    need = (ops.embed_grad_sorted_workspace_bytes(P.grid.numel(), n.attrs["V"], n.channels) if by_sort else
+                            ops.embed_bwd_workspace_bytes(P.grid.numel(), n.channels))
+                    P.embed_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
+                dw = self.grads[n.name + "/weights"]
+                if by_sort:
+                    ops.embed_grad_sorted(P.grid, P.dy[n.name][..., :n.channels], dw, scale=_scale(n), workspace=P.embed_ws)
+                else:
+                    ops.embed_bwd(P.grid, P.dy[n.name][..., :n.channels], dw, P.embed_ws)
                 P.d_embed = P.dy[n.name]
+                P.embed_scale = _scale(n)
         flush()
         if side is not None:
             main.wait_stream(side)     # every weight gradient is in place; the buffers it read may be reused
@@ -722,6 +772,8 @@ class Engine(object):
             # partial rows per layer differ (B x slices of H*W): group the layers by row count
             groups = OrderedDict()
             for n in P.convs:
+                if _group(n):
+                    continue      # no bias; gamma and beta have their gradients from gn_bwd
                 groups.setdefault(P.dbpart[n.name].shape[0], []).append((P.dbpart[n.name], self.grads[n.name + "/biases"]))
             P._sum_rows_batches = [(rows, ops.sum_rows_batched(ents, rows)) for rows, ents in groups.items()]
         else:
@@ -738,36 +790,74 @@ class Engine(object):
         return P
 
     def apply_update(self, P, m, v, lr_t, beta1, beta2, eps, clip, world=1, t=0, emb_rows_sq=None,
-                     scale_growth_interval=1000):
+                     scale_growth_interval=1000, muon=None):
         """The optimizer tail of main_train_json.py:152-156 after loss_backward(defer_l2=True) (and, data parallel, the
         all-reduce): L2 term, tf.clip_by_global_norm, Adam, the repack of the conv operands and the loss-scale update in
         three launches (cutie_opt_norm, cutie_opt_step, cutie_loss_scale_update).  grads_flat holds the SUM of `world`
         replicas' raw gradients.  emb_rows_sq: the embedding rows' share of the squared norm summed over the ranks
         (Trainer.step); None = this replica's, taken inside the first pass.  A step whose norm is not finite (f16
         overflow) or whose conv launches counted a late tile (P.late) changes nothing and is counted in opt_state.
+        muon: None, or a dict(lr, momentum, nesterov, weight_decay, steps): every conv kernel but the logits layer's takes the
+        orthogonalised update (cutie_muon_step, m its momentum, v unused) of the same clipped gradient with its L2 term, under the
+        same skips; the logits layer, the vectors and the embedding stay with Adam.
         Returns the 1-float device tensor of the squared global norm (of the summed gradient)."""
         if not getattr(P, "raw_grads", False):
             raise CutieError("apply_update needs loss_backward(..., defer_l2=True)")
         wd = float(self.net.loss_spec["weight_decay"])
-        if getattr(self, "_opt_layers", None) is None:
+        # which conv kernels Adam takes: all of them, or the logits layer's alone (Trainer keeps to one of the two)
+        if getattr(self, "_opt_layers", None) is None or self._opt_muon != (muon is not None):
             names = sorted(self.conv_w_names, key=lambda k: self.offsets[k][0])
-            self._opt_layers = ops.opt_layers([(self.params[k], self.w_fwd[k], self.w_dg[k]) for k in names])
+            adam = [k for k in names if muon is None or k == self.net.loss_logits_name + "/weights"]
+            self._opt_layers = ops.opt_layers([(self.params[k], self.w_fwd[k], self.w_dg[k]) for k in adam])
             self._opt_partials = torch.zeros(capi.OPT_SCRATCH, dtype=torch.float32, device=self.dev)
+            self._opt_muon = muon is not None
+            self._muon_names = [k for k in names if k not in adam]
+            self._muon_plan = None
         rows = None
         if emb_rows_sq is None and hasattr(P, "d_embed"):
-            rows = P.d_embed.reshape(-1)
+            if P.embed_scale == 1.0:
+                rows = P.d_embed.reshape(-1)
+            else:
+                emb_rows_sq = self.embedding_rows_sumsq(P)      # rows of the table's gradient: scale times d_embed
         ops.opt_norm(self.params_flat, self.grads_flat, self.n_conv_w, self.n_dense, wd * world, self._opt_partials,
                      rows=rows, loss_scale=self.loss_scale)
         ops.opt_step(self.params_flat, self.grads_flat, m, v, self.n_conv_w, wd * world, 0.5 * wd, self._opt_layers, self.dt,
                      lr_t, beta1, beta2, eps, clip, 1.0 / world, t, self._opt_partials, extra_sq=emb_rows_sq,
                      loss_scale=self.opt_state, invalid=P.late, gnorm_sq_out=P.gnorm_sq, reg_out=P.reg,
                      zero_from=self.n_dense)
+        if muon is not None:
+            self._muon_update(P, m, muon, wd * world, clip, 1.0 / world)
         f16 = self.loss_scale is not None
         ops.loss_scale_update(self.opt_state, P.gnorm_sq, backoff=0.5 if f16 else 1.0, growth=2.0 if f16 else 1.0,
                               interval=scale_growth_interval, invalid=P.late)
         P.reg_div, P.l2_pending, P.raw_grads = 1.0, False, False
         self._embed_grad_clean = True      # cutie_opt_step cleared the embedding gradient behind itself
         return P.gnorm_sq
+
+    def _muon_update(self, P, m, hp, l2, clip, grad_scale):
+        """the orthogonalised update of self._muon_names in place, and the repack of their conv operands"""
+        if self._muon_plan is None or self._muon_plan[0] is not m:
+            calls, need = [], 0
+            for lo in range(0, len(self._muon_names), capi.MAX_BATCH):
+                ents = []
+                for k in self._muon_names[lo:lo + capi.MAX_BATCH]:
+                    p, g, mom = self.params[k], self.grads[k], self._view(m, k)
+                    rows, cols = p.numel() // p.shape[-1], p.shape[-1]
+                    ents.append((p, g, mom, p, mom, math.sqrt(max(1.0, cols / rows))))
+                calls.append(ops.muon_descs(ents))
+                need = max(need, ops.orthogonalize_workspace_bytes(calls[-1][1]))
+            self._muon_plan = (m, calls, torch.empty(need, dtype=torch.uint8, device=self.dev) if need else None)
+            self._muon_pack = None
+        _, calls, ws = self._muon_plan
+        for c in calls:
+            ops.muon_step(c, hp["lr"], momentum=hp["momentum"], nesterov=hp["nesterov"], weight_decay=hp["weight_decay"], l2=l2,
+                          steps=hp["steps"], gnorm_sq=P.gnorm_sq, clip=clip, grad_scale=grad_scale, loss_scale=self.opt_state,
+                          invalid=P.late, workspace=ws)
+        if self._muon_pack is None:
+            ents = [(self.params[k], self.w_fwd[k], self.w_dg[k]) for k in self._muon_names]
+            self._muon_pack = ops.pack_weights_batched(ents, self.dt) if ents else []
+        else:
+            ops.replay_pack(self._muon_pack, self.dt, self.dev)
 
     def add_l2_after_reduce(self, P, world=1):
         """Data-parallel tail of loss_backward(on_ready=...): the conv range holds the SUM of the ranks' gradients;
@@ -793,6 +883,8 @@ class Engine(object):
         P.emb_sq.zero_()
         if hasattr(P, "d_embed"):
             ops.sumsq(P.d_embed.reshape(-1), P.emb_sq, P.scratch, self.loss_scale)     # still scaled: activation dtype
+            if P.embed_scale != 1.0:
+                P.emb_sq.mul_(P.embed_scale ** 2)
         return P.emb_sq
 
     def global_norm_sq(self, P, tf_indexed_slices=True, embedding_rows_sq=None):
@@ -804,6 +896,10 @@ class Engine(object):
         if embedding_rows_sq is not None:
             ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
             P.gnorm_sq.add_(embedding_rows_sq)
+        elif tf_indexed_slices and hasattr(P, "d_embed") and P.embed_scale != 1.0:
+            rows = self.embedding_rows_sumsq(P)
+            ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
+            P.gnorm_sq.add_(rows)
         elif tf_indexed_slices and hasattr(P, "d_embed"):
             ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
             ops.sumsq(P.d_embed.reshape(-1), P.gnorm_sq, P.scratch, self.loss_scale)   # still scaled: activation dtype

@@ -21,9 +21,19 @@ from .parallel import GradBuckets, dist_info
 class Trainer(object):
     def __init__(self, engine, learning_rate=1e-4, clip_norm=10.0, beta1=0.9, beta2=0.999, epsilon=1e-8,
                  lr_decay_step=13000, lr_decay_factor=0.1, n_buckets=2, check_inputs=False,
-                 scale_growth_interval=1000, gc_freeze=True):
+                 scale_growth_interval=1000, gc_freeze=True, optimizer="adam", muon_lr=0.02, muon_momentum=0.95, muon_nesterov=True,
+                 muon_weight_decay=0.0, muon_steps=5):
+        """optimizer: 'adam' (the reference's) or 'muon' (no counterpart there): the conv kernels take the orthogonalised update
+        of cutie_muon_step with muon_* (muon_lr decays with learning_rate), the logits layer, the vectors and the embedding
+        Adam as before."""
         self.eng = engine
         self.lr = float(learning_rate)
+        if optimizer not in ("adam", "muon"):
+            raise ValueError("optimizer %r (adam, muon)" % (optimizer,))
+        self.muon = None
+        if optimizer == "muon":
+            self.muon = {"lr": float(muon_lr), "momentum": float(muon_momentum), "nesterov": bool(muon_nesterov),
+                         "weight_decay": float(muon_weight_decay), "steps": int(muon_steps)}
         self.clip, self.b1, self.b2, self.eps = float(clip_norm), beta1, beta2, epsilon
         self.lr_decay_step, self.lr_decay_factor = lr_decay_step, lr_decay_factor
         self.iter = 0          # the reference's `iter` (drives lr decay)
@@ -56,6 +66,8 @@ class Trainer(object):
         eng = self.eng
         if self.iter != 0 and self.lr_decay_step and self.iter % self.lr_decay_step == 0:
             self.lr *= self.lr_decay_factor
+            if self.muon is not None:
+                self.muon["lr"] *= self.lr_decay_factor
         P = eng.forward(batch["grid_table"], image=batch.get("data_image"), ps_1d_indices=batch.get("ps_1d_indices"),
                         labels=batch["gt_classes"])
         if self.check_inputs:
@@ -80,7 +92,8 @@ class Trainer(object):
         # conv tiles that gave up waiting for each other (P.late): the kernel takes them out of the bias correction
         # (opt_state[3]) and leaves everything untouched on such a step; no host read-back
         gn = eng.apply_update(P, self.m, self.v, lr_t, self.b1, self.b2, self.eps, self.clip, world=self.world, t=self.t,
-                              emb_rows_sq=emb_sq, scale_growth_interval=self.scale_growth_interval)
+                              emb_rows_sq=emb_sq, scale_growth_interval=self.scale_growth_interval,
+                              **({} if self.muon is None else {"muon": self.muon}))
         if self.check_inputs:
             eng.check_inputs(P)            # late tiles of the whole step, backward included (the device skipped it already)
         self.iter += 1
