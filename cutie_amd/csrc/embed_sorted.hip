@@ -454,16 +454,19 @@ __global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict_
                                                        const float* __restrict__ slots, const int* __restrict__ starts) {
     __shared__ float sh[JOIN * VEC];
     __shared__ int first;
-    const int64_t w = blockIdx.x;
-    if (starts[w] != 1) return;
-    const unsigned key = pairs[(w + 1) * s.rows * s.L - 1].x;
-    if (key >= (unsigned)s.V) return;
+    const int64_t w = blockIdx.x, tail = min(s.n, (w + 1) * s.rows * s.L) - 1;
     int64_t last = w + 1;
+    // three loads that do not wait for each other
+    const int mine = starts[w];
+    const unsigned key = pairs[tail].x;
+    int next = last + threadIdx.x < s.chunks ? starts[last + threadIdx.x] : 0;
+    if (mine != 1 || key >= (unsigned)s.V) return;
     for (;; last += JOIN) {      // a run that leaves a chunk ends in a later one, so there is a first that is not filled
         if (threadIdx.x == 0) first = JOIN;
         __syncthreads();
         const int64_t k = last + threadIdx.x;
-        if (k >= s.chunks || starts[k] != 2) atomicMin(&first, (int)threadIdx.x);
+        if (last > w + 1) next = k < s.chunks ? starts[k] : 0;
+        if (next != 2) atomicMin(&first, (int)threadIdx.x);
         __syncthreads();
         const int f = first;
         __syncthreads();

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
     if (!flip) {
         // straight through: 16 lanes take a row of 64, four values each
         __syncthreads();
-        const float k = (float)((double)X_SCALE / (sqrt(total) + (double)eps));
+        const double k = (double)X_SCALE / (sqrt(total) + (double)eps);
         const int c = s0 + (threadIdx.x & 15) * 4;
         const bool wide = (M.cols & 3) == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0 && c < M.cols;
 #pragma unroll
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= k;
+            for (int e = 0; e < 4; ++e) v[e] = (float)((double)v[e] * k);      // 1 / norm may leave f32
             store4_split(at(ws, M.y0) + cell(l0 + r, M.Sp, c), v);
         }
         return;
@@ -190,13 +190,13 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
         tile[c][r] = row < M.rows && col < M.cols ? src[(int64_t)row * M.cols + col] : 0.f;
     }
     __syncthreads();
-    const float k = (float)((double)X_SCALE / (sqrt(total) + (double)eps));
+    const double k = (double)X_SCALE / (sqrt(total) + (double)eps);
     const int l = threadIdx.x >> 2, q = (threadIdx.x & 3) * 16;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
         float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = tile[l][q + e + j] * k;
+        for (int j = 0; j < 4; ++j) v[j] = (float)((double)tile[l][q + e + j] * k);
         store4_split(at(ws, M.y0) + cell(l0 + l, M.Sp, s0 + q + e), v);
     }
 }
@@ -626,8 +626,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios 
     __syncthreads();
     sum = part[0];
     for (int w = 1; w < SMALL_WAVES; ++w) sum += part[w];
-    const float k = (float)(1.0 / (sqrt(sum) + (double)eps));
-    for (int i = threadIdx.x; i < L * ld; i += SMALL_THREADS) X[i] *= k;
+    const double k = 1.0 / (sqrt(sum) + (double)eps);
+    for (int i = threadIdx.x; i < L * ld; i += SMALL_THREADS) X[i] = (float)((double)X[i] * k);
     __syncthreads();
     const int sb = S / 16, lb = L / 16;
     for (int step = 0; step < steps; ++step) {

@@ -542,16 +542,18 @@ int cutie_opt_step(float* p, float* g, float* m, float* v, int64_t n, int64_t n_
  * K17  orthogonalised update: an optimizer step for matrices (the conv kernels as [kh*kw*cin][cout]) beside K12's Adam.   No
  *     counterpart in the reference, which has Adam only (main_train_json.py:153).
  * orthogonalize:  X = g / (|g|_F + eps), then `steps` times X <- a X + X (b A + c A A), A = X^T X (X X^T of a wide matrix: the
- *     same map), a = 3.4445, b = -4.7750, c = 2.0315;  out = X, f32.  out may be g.  steps = 1 .. 32, eps > 0.
+ *     same map), a = 3.4445, b = -4.7750, c = 2.0315;  out = X, f32.  steps = 1 .. 32, eps > 0.  An out may be its own g and
+ *     overlaps nothing else of the call.
  * muon_step:  g' = (g / S + l2 * p) * grad_scale * (clip > 0 ? clip / max(sqrt(*gnorm_sq) * grad_scale, clip) : 1)
  *     m_out = momentum * m + g';   u = nesterov ? g' + momentum * m_out : m_out
  *     p_out = p * (1 - lr * weight_decay) - lr * out_scale * orthogonalize(u)
- *     p_out may be p, m_out may be m; nothing else may overlap.  S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq
+ *     p_out may be its own p, m_out its own m; an output overlaps nothing else of the call.  S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq
  *     (nullable; the squared norm with S taken out, as cutie_opt_step leaves it) that is not finite or *invalid != 0 (nullable)
  *     makes p_out = p, m_out = m.
  * The products run on the matrix cores at f32 accuracy: operands are two f16 (22 bits), sums f32, sums of squares f64, all in
- * a fixed order: the same bits every run for one list of shapes.  X is kept to 2^-36: of a matrix whose norm is below eps, so
- * much less of the (small) result is left.
+ * a fixed order: the same bits every run for one list of shapes (a matrix's bits depend on the others of its call: K is cut by their number).  X is kept to 2^-36 there: of a matrix whose norm lies
+ * far below eps, less of the (then small) result is left.  A matrix of up to 64 x 192 values (either way round) is computed by one
+ * workgroup in f32.
  * Matrices are contiguous f32 [rows][cols], any size from 1 x 1 to 2^29 values (padded to multiples of 64), up to
  * CUTIE_MAX_BATCH a call, in one set of launches.  descs / shapes (rows, cols of each matrix) are HOST arrays.
  * workspace: cutie_orthogonalize_workspace_bytes(shapes, n) bytes for the same shapes in the same order, 256-byte aligned,

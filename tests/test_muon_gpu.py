@@ -89,7 +89,7 @@ def matrix(r, c, kind, g):
 
 SIZES = [(1, 1), (1, 7), (9, 1), (2, 2), (18, 64), (64, 18), (63, 65), (64, 64), (65, 129), (128, 128), (300, 129), (256, 1000),
          (1920, 256), (130, 4000), (700, 700),
-         (192, 64), (64, 192), (193, 64), (64, 193), (192, 65), (3000, 20), (520, 530)]      # both sides of the one-workgroup form
+         (192, 64), (64, 192), (193, 64), (64, 193), (192, 65), (3000, 20), (520, 530), (1, 2500), (2500, 1)]      # both sides of the one-workgroup form
 
 
 @pytest.mark.gpu
@@ -120,11 +120,12 @@ def test_many_tiles(r, c):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("steps", [1, 2, 3, 6])
-def test_steps(steps):
-    u = matrix(70, 40, "falling", torch.Generator().manual_seed(1))
+@pytest.mark.parametrize("steps", [1, 2, 3, 6, 12])
+@pytest.mark.parametrize("r,c", [(70, 40), (300, 70)])
+def test_steps(r, c, steps):
+    u = matrix(r, c, "falling", torch.Generator().manual_seed(1))
     want, tol = allowed(u, steps)
-    out = torch.empty(70, 40, device=DEV)
+    out = torch.empty(r, c, device=DEV)
     ops.orthogonalize_batched([(u.to(DEV), out)], steps=steps)
     assert float((out.cpu().double() - want).norm()) <= tol
 
@@ -159,20 +160,25 @@ def test_singular_values_and_shapes_of_filters():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("mag", [1e-25, 1e-4, 1e25])
-def test_magnitudes(mag):
+@pytest.mark.parametrize("mag", [1e-25, 1e-4, 1e25, 5e37])
+@pytest.mark.parametrize("r,c", [(50, 80), (300, 200)])
+def test_magnitudes(r, c, mag):
     """the squares of the values leave f32: the norm is f64, and the result does not depend on the scale"""
-    u = matrix(50, 80, "normal", torch.Generator().manual_seed(6)) * mag
+    u = matrix(r, c, "normal", torch.Generator().manual_seed(6)) * mag
     want, tol = allowed(u, eps=1e-30)
-    out = torch.empty(50, 80, device=DEV)
+    assert bool(torch.isfinite(u).all())
+    out = torch.empty(r, c, device=DEV)
     ops.orthogonalize_batched([(u.to(DEV), out)], eps=1e-30)
     assert float((out.cpu().double() - want).norm()) <= tol
 
 
 @pytest.mark.gpu
 def test_zero_small_and_not_finite():
-    z = torch.zeros(70, 30, device=DEV)
-    out = torch.full_like(z, 7.0)
+    for shape in ((70, 30), (300, 70)):
+        z = torch.zeros(shape, device=DEV)
+        out = torch.full_like(z, 7.0)
+        ops.orthogonalize_batched([(z, out)], eps=1e-38)
+        assert bool((out == 0).all())
     bad = torch.randn(40, 40, device=DEV)
     bad[3, 3] = float("nan")
     good = torch.randn(66, 40, generator=torch.Generator().manual_seed(1)).to(DEV)
