@@ -81,7 +81,8 @@ __global__ __launch_bounds__(256) void embed_scaled_kernel(const int32_t* __rest
 
 // ------------------------------------------------------------------------------------------------------------------- sort
 constexpr int ITEMS = 4;                // elements a thread ranks in the many-tile form
-constexpr int TILE = 256 * ITEMS;       // elements a workgroup ranks there
+constexpr int TILE = 1024 * ITEMS;      // elements a workgroup ranks there
+constexpr int SELF_TILES = 128;         // up to so many tiles a tile adds up the counts before it by itself; more take sort_scan_kernel
 constexpr int ONE = 1024 * 8;           // elements one workgroup sorts by itself (4 or 8 a thread)
 constexpr int MAX_BITS = 10, MAX_BINS = 1 << MAX_BITS;
 
@@ -218,11 +219,11 @@ __global__ __launch_bounds__(1024) void sort_one_kernel(const int32_t* __restric
 
 // counts[tile][bin] of one digit
 template <bool FIRST>
-__global__ __launch_bounds__(256) void sort_count_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
+__global__ __launch_bounds__(1024) void sort_count_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
                                                          int shift, int bits, unsigned* __restrict__ counts) {
     __shared__ unsigned hist[4][MAX_BINS];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
-    for (int i = threadIdx.x; i < 4 * bins; i += 256) hist[i >> bits][i & (bins - 1)] = 0;
+    for (int i = threadIdx.x; i < 4 * bins; i += 1024) hist[i >> bits][i & (bins - 1)] = 0;
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r) {
@@ -232,10 +233,10 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const int32_t* __restri
         if (ok) key = FIRST ? first_pair(ids, i, V).x : in[i].x;
         const unsigned d = (key >> shift) & (bins - 1);
         const unsigned long long m = same_digit(d, bits, __ballot(ok));
-        if (ok && (m & ((1ull << lane) - 1)) == 0) atomicAdd(&hist[w][d], (unsigned)__popcll(m));
+        if (ok && (m & ((1ull << lane) - 1)) == 0) atomicAdd(&hist[w & 3][d], (unsigned)__popcll(m));
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += 256)
+    for (int b = threadIdx.x; b < bins; b += 1024)
         counts[((int64_t)blockIdx.x << bits) + b] = hist[0][b] + hist[1][b] + hist[2][b] + hist[3][b];
 }
 
@@ -272,12 +273,13 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(unsigned* __restrict__ 
     }
 }
 
+// totals NULL: counts are the tiles' own, and each tile adds them up; else as sort_scan_kernel left them
 template <bool FIRST>
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
-                                                           int shift, int bits, const unsigned* __restrict__ counts,
-                                                           const unsigned* __restrict__ totals, uint2* __restrict__ out) {
-    __shared__ unsigned short cnt[4][MAX_BINS];
-    __shared__ unsigned base[MAX_BINS];
+__global__ __launch_bounds__(1024) void sort_scatter_kernel(const int32_t* __restrict__ ids, const uint2* __restrict__ in, int64_t n, int V,
+                                                            int shift, int bits, const unsigned* __restrict__ counts,
+                                                            const unsigned* __restrict__ totals, uint2* __restrict__ out) {
+    __shared__ unsigned short cnt[16][MAX_BINS];
+    __shared__ unsigned base[MAX_BINS], before[MAX_BINS];
     __shared__ unsigned wsum[4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, bins = 1 << bits;
     uint2 p[ITEMS];
@@ -291,10 +293,29 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const int32_t* __rest
         p[r] = !ok[r] ? make_uint2(0, 0) : (FIRST ? first_pair(ids, i, V) : in[i]);
         d[r] = (p[r].x >> shift) & (bins - 1);
     }
-    for (int b = threadIdx.x; b < bins; b += 256) base[b] = totals[b];
-    bin_scan<256>(base, bins, wsum);
-    for (int b = threadIdx.x; b < bins; b += 256) base[b] += counts[((int64_t)blockIdx.x << bits) + b];
-    tile_rank<4, ITEMS>(d, ok, bits, cnt, rank, nullptr);
+    if (totals) {
+        for (int b = threadIdx.x; b < bins; b += 1024) {
+            base[b] = totals[b];
+            before[b] = counts[((int64_t)blockIdx.x << bits) + b];
+        }
+    } else {
+        for (int b = threadIdx.x; b < bins; b += 1024) base[b] = before[b] = 0;
+        __syncthreads();
+        // 1024 / bins groups of threads take every so many tiles; whole numbers, so the order of the additions is no matter
+        const int groups = 1024 >> bits, b = threadIdx.x & (bins - 1), tiles = gridDim.x;
+        unsigned all = 0, early = 0;
+#pragma unroll 8
+        for (int t = threadIdx.x >> bits; t < tiles; t += groups) {
+            const unsigned c = counts[((int64_t)t << bits) + b];
+            all += c;
+            early += t < (int)blockIdx.x ? c : 0u;
+        }
+        if (all) atomicAdd(&base[b], all);
+        if (early) atomicAdd(&before[b], early);
+    }
+    bin_scan<1024>(base, bins, wsum);
+    for (int b = threadIdx.x; b < bins; b += 1024) base[b] += before[b];
+    tile_rank<16, ITEMS>(d, ok, bits, cnt, rank, nullptr);
 #pragma unroll
     for (int r = 0; r < ITEMS; ++r)
         if (ok[r]) out[base[d[r]] + rank[r]] = p[r];
@@ -645,10 +666,12 @@ extern "C" int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, cons
             const int shift = pass * sp.bits;
             auto count = pass ? sort_count_kernel<false> : sort_count_kernel<true>;
             auto scatter = pass ? sort_scatter_kernel<false> : sort_scatter_kernel<true>;
-            hipLaunchKernelGGL(count, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)cdiv(bins, 16)), dim3(1024), 0, stream, counts, sp.tiles, sp.bits, totals);
-            hipLaunchKernelGGL(scatter, dim3((unsigned)sp.tiles), dim3(256), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts, totals,
-                               out);
+            const bool scan = sp.tiles > SELF_TILES;
+            hipLaunchKernelGGL(count, dim3((unsigned)sp.tiles), dim3(1024), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts);
+            if (scan)
+                hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)cdiv(bins, 16)), dim3(1024), 0, stream, counts, sp.tiles, sp.bits, totals);
+            hipLaunchKernelGGL(scatter, dim3((unsigned)sp.tiles), dim3(1024), 0, stream, ids, in, n_cells, V, shift, sp.bits, counts,
+                               scan ? totals : nullptr, out);
             CUTIE_CHECK_LAUNCH();
         }
         sorted = buf[(sp.passes - 1) & 1];

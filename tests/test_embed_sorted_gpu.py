@@ -82,7 +82,8 @@ CASES = [
     (65536, 3000, 40, 0, 0, "grid"), (65537, 1 << 20, 16, 0, 0, "uniform"), (65537, (1 << 20) + 1, 8, 0, 0, "uniform"),
     (131072, 18000, 128, 64, 0, "grid"), (262145, 18000, 24, 0, 0, "one"),
     (3000, 50, 2048, 0, 0, "grid"), (3000, 50, 2052, 0, 0, "grid"), (700, 50, 1031, 2, 0, "grid"),
-    (30000, 50, 1, 0, 0, "uniform"), (30000, 2, 2, 0, 0, "grid"),
+    (30000, 50, 1, 0, 0, "uniform"), (30000, 2, 2, 0, 0, "grid"), (12288, 40, 8, 0, 0, "falling"), (12289, 1000, 8, 0, 0, "outside"),
+    (524288, 3000, 4, 0, 0, "rising"), (524289, 3000, 4, 0, 0, "grid"), (700001, 70000, 4, 0, 0, "outside"),      # many tiles
 ]
 
 
