@@ -554,17 +554,22 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Star
 }
 
 // ------------------------------------------------------------------------------------------------------------------- small
-// A matrix with S <= SMALL_S and L <= SMALL_L: one workgroup does everything, X, A and B as f32 in LDS, the products on the f32
-// matrix cores (16 x 16 x 4; they have a sixteenth of the f16 rate, but the launches of the general form alone take longer).  Five
-// steps: 16 x 16 9 us, 64 x 18 19, 128 x 64 59, 256 x 64 102; the general form takes 82 at 257 x 64.
-constexpr int SMALL_S = 64, SMALL_L = 192, SMALL_THREADS = 512, SMALL_WAVES = SMALL_THREADS / 64;
-inline bool is_small(int r, int c) { return (r > c ? c : r) <= SMALL_S && (r > c ? r : c) <= SMALL_L; }
+// Matrices of few rows and columns: one workgroup does everything, X, A and B as f32 in LDS, the products on the f32 matrix cores
+// (16 x 16 x 4; they have a sixteenth of the f16 rate, but the launches of the general form alone take longer).  The limit is where
+// the tall form below takes as long.  Five steps, one matrix: 128 x 16 17 us (tall 36), 352 x 16 35 (39), 64 x 18 18,
+// 288 x 32 48 (42), 192 x 48 61 (53), 128 x 64 56 (66), 192 x 64 80 (67).
+constexpr int SMALL_S = 64, SMALL_THREADS = 512, SMALL_WAVES = SMALL_THREADS / 64;
+constexpr int TALL_L = 8192;
 __host__ __device__ inline int up16(int v) { return (v + 15) & ~15; }
+inline bool is_small(int r, int c) {
+    const int L = r > c ? r : c, S = r > c ? c : r;
+    return S <= SMALL_S && L <= 384 && L * up16(S) <= 8192;
+}
 inline size_t small_lds(int r, int c) {
     const int L = up16(r > c ? r : c), S = up16(r > c ? c : r), ld = S + 4;
     return ((size_t)L + 2 * S) * ld * sizeof(float);
 }
-struct Smalls { int rows[CUTIE_MAX_BATCH], cols[CUTIE_MAX_BATCH]; };
+struct Smalls { int rows[CUTIE_MAX_BATCH], cols[CUTIE_MAX_BATCH], n; };
 
 // acc[c] += P(row m, k) Q(k, column n) over k = 0 .. K-1 for NC column blocks: pa = P's address of (m = li, k = lg), pk its
 // step per k; qa = Q's address of (k = lg, n = li), qk likewise
@@ -586,6 +591,48 @@ __device__ __forceinline__ void small_product(const float* pa, int pk, const flo
     }
 }
 
+// dst = X^T X over L rows, 16 x 16 blocks round the waves; a lane ends with rows lg * 4 .. of one column
+__device__ __forceinline__ void small_gram(const float* X, int ld, int L, int S, float* dst, int ldd, int waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, sb = S / 16;
+    for (int t = wave; t < sb * sb; t += waves) {
+        const int m0 = t / sb * 16, n0 = t % sb * 16;
+        float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
+        small_product<1>(X + lg * ld + m0 + li, ld, X + lg * ld + n0 + li, ld, L, 1, acc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[(m0 + lg * 4 + e) * ldd + n0 + li] = acc[0][e];
+    }
+}
+// B = a I + b A + c A A
+__device__ __forceinline__ void small_b(const float* A, float* B, int ld, int S, int waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, sb = S / 16;
+    for (int t = wave; t < sb * sb; t += waves) {
+        const int m0 = t / sb * 16, n0 = t % sb * 16;
+        float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
+        small_product<1>(A + (m0 + li) * ld + lg, 1, A + lg * ld + n0 + li, ld, S, 1, acc);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int m = m0 + lg * 4 + e, n = n0 + li;
+            B[m * ld + n] = fmaf(NS_B, A[m * ld + n], NS_C * acc[0][e]) + (m == n ? NS_A : 0.f);
+        }
+    }
+}
+// X = X B in place: a wave's 16 rows depend on themselves alone
+__device__ __forceinline__ void small_apply(float* X, const float* B, int ld, int L, int S, int waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4, sb = S / 16;
+    for (int t = wave; t < L / 16; t += waves) {
+        float4_t acc[SMALL_S / 16];
+#pragma unroll
+        for (int c = 0; c < SMALL_S / 16; ++c) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+        small_product<SMALL_S / 16>(X + (t * 16 + li) * ld + lg, 1, B + lg * ld + li, ld, S, sb, acc);
+#pragma unroll
+        for (int c = 0; c < SMALL_S / 16; ++c)
+            if (c < sb) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) X[(t * 16 + lg * 4 + e) * ld + c * 16 + li] = acc[c][e];
+            }
+    }
+}
+
 template <bool MUON>
 __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios ios, Hyper h, int steps, float eps) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -597,7 +644,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios 
     float* X = lds;                // [L][ld]
     float* A = X + L * ld;         // [S][ld]
     float* B = A + S * ld;         // [S][ld]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool skip = MUON && skip_step(h);
     float inv = 1.f, scale = 1.f;
     if constexpr (MUON) {
@@ -629,42 +676,12 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios 
     const double k = 1.0 / (sqrt(sum) + (double)eps);
     for (int i = threadIdx.x; i < L * ld; i += SMALL_THREADS) X[i] = (float)((double)X[i] * k);
     __syncthreads();
-    const int sb = S / 16, lb = L / 16;
     for (int step = 0; step < steps; ++step) {
-        // A = X^T X, 16 x 16 blocks round the waves; a lane ends with rows lg * 4 .. of one column
-        for (int t = wave; t < sb * sb; t += SMALL_WAVES) {
-            const int m0 = t / sb * 16, n0 = t % sb * 16;
-            float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
-            small_product<1>(X + lg * ld + m0 + li, ld, X + lg * ld + n0 + li, ld, L, 1, acc);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) A[(m0 + lg * 4 + e) * ld + n0 + li] = acc[0][e];
-        }
+        small_gram(X, ld, L, S, A, ld, SMALL_WAVES);
         __syncthreads();
-        // B = a I + b A + c A A
-        for (int t = wave; t < sb * sb; t += SMALL_WAVES) {
-            const int m0 = t / sb * 16, n0 = t % sb * 16;
-            float4_t acc[1] = {float4_t{0.f, 0.f, 0.f, 0.f}};
-            small_product<1>(A + (m0 + li) * ld + lg, 1, A + lg * ld + n0 + li, ld, S, 1, acc);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int m = m0 + lg * 4 + e, n = n0 + li;
-                B[m * ld + n] = fmaf(NS_B, A[m * ld + n], NS_C * acc[0][e]) + (m == n ? NS_A : 0.f);
-            }
-        }
+        small_b(A, B, ld, S, SMALL_WAVES);
         __syncthreads();
-        // X = X B: a wave's 16 rows depend on themselves alone
-        for (int t = wave; t < lb; t += SMALL_WAVES) {
-            float4_t acc[SMALL_S / 16];
-#pragma unroll
-            for (int c = 0; c < SMALL_S / 16; ++c) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-            small_product<SMALL_S / 16>(X + (t * 16 + li) * ld + lg, 1, B + lg * ld + li, ld, S, sb, acc);
-#pragma unroll
-            for (int c = 0; c < SMALL_S / 16; ++c)
-                if (c < sb) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) X[(t * 16 + lg * 4 + e) * ld + c * 16 + li] = acc[c][e];
-                }
-        }
+        small_apply(X, B, ld, L, S, SMALL_WAVES);
         __syncthreads();
     }
     for (int i = threadIdx.x; i < rows * cols; i += SMALL_THREADS) {
@@ -679,48 +696,256 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios 
     }
 }
 
+// -------------------------------------------------------------------------------------------------------------------- tall
+// S <= SMALL_S and L <= TALL_L: tiles of rows, one workgroup each, f32 products as above.  The first launch makes U and each
+// tile's part of U^T U; a step is one launch, in which every workgroup adds up all parts of A, makes B, takes its rows of X through
+// it and, for the step after, makes its part of X'^T X': 1 + steps launches in place of the general form's 2 + 4 steps.
+// One matrix, five steps: 3 x 3552 45 us (general form 112), 1024 x 64 73 (120), 5634 x 42 87 (163), 8192 x 64 136 (187), of which
+// the launches alone take 30.  At S = 64 the rest is the f32 matrix cores and, with 32 tiles, each workgroup's 512 KB of parts.
+constexpr int TALL_TILES = 32, TALL_ROWS = 64;
+struct Tall { int rows, cols, R, tiles, y, slab, head; };      // y [tiles R][S], slab [2][tiles][S][S], head [tiles]
+struct Talls { Tall t[CUTIE_MAX_BATCH]; int n; };
+// of a tile of U: the sum of squares, and the power of two above its largest value, by which U is divided in its part of U^T U: squares
+// of any f32 stay in range
+struct Head { double sum; int exp, pad; };
+
+// X (LDS, [R][ld]) <-> y's rows
+template <int T> __device__ __forceinline__ void tall_store(const float* X, float* y, int R, int S, int ld) {
+    const int q = S / 4;
+    for (int i = threadIdx.x; i < R * q; i += T) {
+        const int r = i / q, c = (i - r * q) * 4;
+        *reinterpret_cast<float4*>(y + (int64_t)r * S + c) = *reinterpret_cast<const float4*>(X + r * ld + c);
+    }
+}
+
+// A = sum of the tiles' parts, those of the first step times ratio ** 2.  N loads are on their way together; `groups` neighbouring
+// lanes (a power of two at S = 16 and 32, else one) share four values.
+template <int N, int T>
+__device__ __forceinline__ void tall_fold(float* A, const float* slab, const float* ratio, int tiles, int S, int ld, bool first) {
+    const int q = S / 4, quads = S * q, groups = S > 32 || quads >= T ? 1 : T / quads, per = (tiles + groups - 1) / groups;
+    for (int k = threadIdx.x; k < quads * groups; k += T) {
+        const int c4 = k / groups, t0 = (k - c4 * groups) * per, t1 = min(tiles, t0 + per);
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int t = t0; t < t1; t += N) {
+            float4_t w[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = *reinterpret_cast<const float4_t*>(slab + c4 * 4 + (int64_t)min(t + j, t1 - 1) * S * S);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (t + j >= t1) continue;
+                if (first) w[j] = w[j] * ratio[t + j] * ratio[t + j];
+                v += w[j];
+            }
+        }
+        for (int o = 1; o < groups; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
+        const int r = c4 / q, c = (c4 - r * q) * 4;
+        if (t0 == 0) *reinterpret_cast<float4_t*>(A + r * ld + c) = v;
+    }
+}
+
+template <int T, bool MUON>
+__global__ __launch_bounds__(T) void ns_tall_start_kernel(Talls ts, Ios ios, Starts st, Hyper h, char* ws) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    __shared__ double part[T / 64];
+    __shared__ float top[T / 64];
+    const int i = find(st, ts.n, blockIdx.x), tile = blockIdx.x - st.v[i];
+    const Tall M = ts.t[i];
+    const Io io = ios.io[i];
+    const bool flip = M.rows < M.cols;
+    const int L = flip ? M.cols : M.rows, s = flip ? M.rows : M.cols, S = up16(s), ld = S + 4;
+    const int l0 = tile * M.R, live = min(M.R, L - l0);      // the plan leaves no tile empty
+    float* X = lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool skip = MUON && skip_step(h);
+    float inv = 1.f, scale = 1.f;
+    if constexpr (MUON) {
+        inv = h.loss_scale ? h.loss_scale[1] : 1.f;
+        scale = clip_scale(h);
+    }
+    for (int k = threadIdx.x; k < M.R * ld; k += T) X[k] = 0.f;
+    __syncthreads();
+    double sum = 0;
+    float big = 0.f;
+    for (int k = threadIdx.x; k < live * s; k += T) {
+        // along the caller's rows
+        const int a = flip ? k / live : k / s, b = flip ? k - a * live : k - a * s;
+        const int64_t e = flip ? (int64_t)a * M.cols + l0 + b : (int64_t)l0 * s + k;
+        float v;
+        if constexpr (MUON) {
+            const float g = (io.g[e] * inv + h.l2 * io.p[e]) * scale, m0 = io.m[e], m1 = h.mu * m0 + g;
+            v = h.nesterov ? g + h.mu * m1 : m1;
+            io.mo[e] = skip ? m0 : m1;
+        } else {
+            v = io.g[e];
+        }
+        X[flip ? b * ld + a : a * ld + b] = v;
+        big = fmaxf(big, fabsf(v));
+        sum = fma((double)v, (double)v, sum);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        sum += __shfl_xor(sum, o, 64);
+        big = fmaxf(big, __shfl_xor(big, o, 64));
+    }
+    if (lane == 0) { part[wave] = sum; top[wave] = big; }
+    __syncthreads();
+    sum = part[0];
+    big = top[0];
+    for (int w = 1; w < T / 64; ++w) { sum += part[w]; big = fmaxf(big, top[w]); }
+    int exp = -200;      // of a tile of zeros: its part counts nothing whatever 1 / eps is
+    if (big > 0.f && big <= 3.4028235e38f) (void)frexpf(big, &exp);
+    tall_store<T>(X, (float*)at(ws, M.y) + (int64_t)l0 * S, M.R, S, ld);
+    __syncthreads();
+    for (int k = threadIdx.x; k < M.R * ld; k += T) X[k] = ldexpf(X[k], -exp);
+    __syncthreads();
+    small_gram(X, ld, M.R, S, (float*)at(ws, M.slab) + (int64_t)tile * S * S, S, T / 64);
+    if (threadIdx.x == 0) ((Head*)at(ws, M.head))[tile] = Head{sum, exp, 0};
+}
+
+template <int T, bool MUON>
+__global__ __launch_bounds__(T) void ns_tall_step_kernel(Talls ts, Ios ios, Starts st, Hyper h, int step, int last, float eps, char* ws) {
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    __shared__ float ratio[TALL_TILES];
+    const int i = find(st, ts.n, blockIdx.x), tile = blockIdx.x - st.v[i];
+    const Tall M = ts.t[i];
+    const bool flip = M.rows < M.cols;
+    const int L = flip ? M.cols : M.rows, s = flip ? M.rows : M.cols, S = up16(s), ld = S + 4, q = S / 4;
+    const int l0 = tile * M.R, live = min(M.R, L - l0);
+    float *X = lds, *A = X + M.R * ld, *B = A + S * ld;
+    float* y = (float*)at(ws, M.y) + (int64_t)l0 * S;
+    double k0 = 1.0;
+    if (step == 0) {
+        const Head* head = (const Head*)at(ws, M.head);
+        double total = 0;
+        for (int t = 0; t < M.tiles; ++t) total += head[t].sum;
+        k0 = 1.0 / (sqrt(total) + (double)eps);
+        if (threadIdx.x < M.tiles) ratio[threadIdx.x] = (float)ldexp(k0, head[threadIdx.x].exp);
+        __syncthreads();
+    }
+    for (int k = threadIdx.x; k < M.R * q; k += T) {
+        const int r = k / q, c = (k - r * q) * 4;
+        float4 v = *reinterpret_cast<const float4*>(y + (int64_t)r * S + c);
+        if (step == 0) v = make_float4((float)(v.x * k0), (float)(v.y * k0), (float)(v.z * k0), (float)(v.w * k0));
+        *reinterpret_cast<float4*>(X + r * ld + c) = v;
+    }
+    // A: the tiles' parts, in order
+    const float* slab = (const float*)at(ws, M.slab) + (int64_t)(step & 1) * M.tiles * S * S;
+    if (S > 32) tall_fold<16, T>(A, slab, ratio, M.tiles, S, ld, step == 0);
+    else tall_fold<4, T>(A, slab, ratio, M.tiles, S, ld, step == 0);
+    __syncthreads();
+    small_b(A, B, ld, S, T / 64);
+    __syncthreads();
+    small_apply(X, B, ld, M.R, S, T / 64);
+    __syncthreads();
+    if (!last) {
+        tall_store<T>(X, y, M.R, S, ld);
+        small_gram(X, ld, M.R, S, (float*)at(ws, M.slab) + ((int64_t)((step + 1) & 1) * M.tiles + tile) * S * S, S, T / 64);
+        return;
+    }
+    const Io io = ios.io[i];
+    const bool skip = MUON && skip_step(h);
+    for (int k = threadIdx.x; k < live * s; k += T) {
+        const int a = flip ? k / live : k / s, b = flip ? k - a * live : k - a * s;
+        const int64_t e = flip ? (int64_t)a * M.cols + l0 + b : (int64_t)l0 * s + k;
+        const float v = X[flip ? b * ld + a : a * ld + b];
+        if constexpr (MUON) {
+            const float p = io.p[e];
+            io.po[e] = skip ? p : p * (1.f - h.lr * h.wd) - h.lr * io.k * v;
+        } else {
+            io.po[e] = v;
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------------- host
+// All matrices of a call are computed in one form, the cheapest that takes every one of them: a matrix more in a form's launches costs
+// little, the launches of a second form come on top (14 filters of which one is 7680 x 64 and one 64 x 18: 475 us with those two in
+// launches of their own forms 575).
 struct NsPlan {
-    Mats ms;                 // the matrices of the general form
-    Smalls sm;               // those of the small one
-    int n_small, order[CUTIE_MAX_BATCH];      // the caller's index of each: the general ones, then the small ones
-    size_t lds;              // of the small form
+    enum { SMALL, TALL, GENERAL } form;
+    Mats ms;                 // GENERAL
+    Smalls sm;               // SMALL
+    Talls tall;              // TALL
+    size_t lds;              // of SMALL and TALL
+    bool tall_wide;          // a tall one has S > 32
     Splits gram, square;
     bool fold_square;        // some A A is cut along K
     int fg, fs, fa;          // tile factors (4: 128 x 128, 2: 64 x 64) of the three products
     size_t bytes;
 };
 
+// rows of a tile of the tall form: 64 or, where that makes more than TALL_TILES tiles (all of whose parts every workgroup reads), more
+inline int tall_rows(int L) {
+    int64_t tiles = cdiv(L, TALL_ROWS);
+    return up16((int)cdiv(L, tiles > TALL_TILES ? TALL_TILES : tiles));
+}
+
 inline int tri_tiles(int Sp, int f) { const int nt = (int)cdiv(Sp, 32 * f); return nt * (nt + 1) / 2; }
 
 // shapes: (rows, cols) of n matrices
 inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
     CUTIE_CHECK_ARG(n >= 1 && n <= CUTIE_MAX_BATCH, "%s: %d matrices (1..%d)", who, n, CUTIE_MAX_BATCH);
-    p.ms.n = p.n_small = 0;
-    p.fold_square = false;
+    p.fold_square = p.tall_wide = false;
+    p.form = NsPlan::SMALL;
     p.lds = 0;
+    int64_t broad = 0;      // workgroups of the tall form with S = 64
+    for (int i = 0; i < n; ++i) {
+        const int r = shapes[2 * i], c = shapes[2 * i + 1], L = r > c ? r : c, S = r > c ? c : r;
+        CUTIE_CHECK_ARG(r >= 1 && c >= 1, "%s: matrix %d is %d x %d", who, i, r, c);
+        if (S > SMALL_S || L > TALL_L) p.form = NsPlan::GENERAL;
+        else if (p.form == NsPlan::SMALL && !is_small(r, c)) p.form = NsPlan::TALL;
+        if (S > 48) broad += cdiv(L, tall_rows(L));
+    }
+    // One round of workgroups: at S = 64 the f32 products of more take longer than the general form (8192 x 64: 4 matrices 151 us,
+    // general 231; 32 matrices 711, general 453.  At S = 48 32 of 7079 x 35 take 343, general 478)
+    if (p.form == NsPlan::TALL && broad > 256) p.form = NsPlan::GENERAL;
+    size_t off = 0;      // of the workspace, in units of 256 bytes
+    auto take = [&](int64_t bytes) {
+        const size_t at = off;
+        off += (size_t)cdiv(bytes, 256);
+        return (int)at;
+    };
+    p.sm.n = p.tall.n = p.ms.n = n;
+    if (p.form == NsPlan::SMALL) {
+        for (int i = 0; i < n; ++i) {
+            p.sm.rows[i] = shapes[2 * i];
+            p.sm.cols[i] = shapes[2 * i + 1];
+            const size_t lds = small_lds(p.sm.rows[i], p.sm.cols[i]);
+            if (lds > p.lds) p.lds = lds;
+        }
+        p.bytes = 256;      // none needed; a size all the same
+        return CUTIE_OK;
+    }
+    if (p.form == NsPlan::TALL) {
+        for (int i = 0; i < n; ++i) {
+            const int r = shapes[2 * i], c = shapes[2 * i + 1], L = r > c ? r : c, S = up16(r > c ? c : r);
+            Tall& t = p.tall.t[i];
+            t.rows = r;
+            t.cols = c;
+            t.R = tall_rows(L);
+            t.tiles = (int)cdiv(L, t.R);
+            t.y = take((int64_t)t.tiles * t.R * S * 4);
+            t.slab = take((int64_t)2 * t.tiles * S * S * 4);
+            t.head = take((int64_t)t.tiles * sizeof(Head));
+            const size_t lds = ((size_t)t.R + 2 * S) * (S + 4) * sizeof(float);
+            if (lds > p.lds) p.lds = lds;
+            if (S > 32) p.tall_wide = true;
+        }
+        p.bytes = off * 256;
+        return CUTIE_OK;
+    }
     for (int i = 0; i < n; ++i) {
         const int r = shapes[2 * i], c = shapes[2 * i + 1];
-        CUTIE_CHECK_ARG(r >= 1 && c >= 1, "%s: matrix %d is %d x %d", who, i, r, c);
-        if (is_small(r, c)) continue;
         const int64_t Lp = cdiv(r > c ? r : c, 64) * 64, Sp = cdiv(r > c ? c : r, 64) * 64;
         CUTIE_CHECK_ARG(Lp * Sp < ((int64_t)1 << 29), "%s: matrix %d is %d x %d (padded to multiples of 64, below 2^29 values)", who, i, r, c);
-        Mat& m = p.ms.m[p.ms.n];
+        Mat& m = p.ms.m[i];
         m.rows = r;
         m.cols = c;
         m.Lp = (int)Lp;
         m.Sp = (int)Sp;
-        p.order[p.ms.n++] = i;
     }
-    for (int i = 0; i < n; ++i) {
-        const int r = shapes[2 * i], c = shapes[2 * i + 1];
-        if (!is_small(r, c)) continue;
-        p.sm.rows[p.n_small] = r;
-        p.sm.cols[p.n_small] = c;
-        p.order[p.ms.n + p.n_small++] = i;
-        if (small_lds(r, c) > p.lds) p.lds = small_lds(r, c);
-    }
-    n = p.ms.n;
     // The 128 tile where it gives every CU a workgroup, K cut into pieces of eight steps where it can be (14 filters: 475 us; with
     // the 64 tile for X B 526, for X^T X 532); two workgroups a CU by cutting K (512 / tiles: 475 us, 256 530, 1024 538)
     int64_t tg = 0, ts = 0, ta = 0;
@@ -734,14 +959,7 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
     p.fs = ts >= 256 ? 4 : 2;
     p.fa = ta >= 256 ? 4 : 2;
     int64_t ng = 0, nq = 0;
-    if (!n) { p.bytes = 256; return CUTIE_OK; }      // no workspace needed; a size all the same
     for (int i = 0; i < n; ++i) { ng += tri_tiles(p.ms.m[i].Sp, p.fg); nq += tri_tiles(p.ms.m[i].Sp, p.fs); }
-    size_t off = 0;
-    auto take = [&](int64_t bytes) {
-        const size_t at = off;
-        off += (size_t)cdiv(bytes, 256);
-        return (int)at;
-    };
     for (int i = 0; i < n; ++i) {
         Mat& m = p.ms.m[i];
         auto cut = [](int64_t want, int steps) {      // at least four K steps a part
@@ -795,19 +1013,43 @@ inline void ns_apply(const NsPlan& p, const Ios& ios, const Hyper& h, int which,
     else hipLaunchKernelGGL((ns_apply_kernel<F, false, false>), dim3(g), dim3(256), 0, stream, p.ms, ios, st, h, which, ws);
 }
 
-template <bool MUON>
-inline int ns_run(const NsPlan& p, const Ios& given, const Hyper& h, int steps, float eps, char* ws, hipStream_t stream) {
-    static_assert(sizeof(Mats) + sizeof(Ios) + sizeof(Starts) + sizeof(Hyper) + 64 < 4096, "kernel arguments");
-    Ios ios = {};
-    if (p.n_small) {
-        for (int i = 0; i < p.n_small; ++i) ios.io[i] = given.io[p.order[p.ms.n + i]];
-        CUTIE_ENSURE_LDS(ns_small_kernel<MUON>, p.lds);
-        hipLaunchKernelGGL((ns_small_kernel<MUON>), dim3((unsigned)p.n_small), dim3(SMALL_THREADS), p.lds, stream, p.sm, ios, h, steps, eps);
+template <int T, bool MUON>
+inline int ns_tall(const NsPlan& p, const Ios& ios, const Starts& st, const Hyper& h, int wgs, int steps, float eps, char* ws, hipStream_t stream) {
+    CUTIE_ENSURE_LDS((ns_tall_start_kernel<T, MUON>), p.lds);
+    CUTIE_ENSURE_LDS((ns_tall_step_kernel<T, MUON>), p.lds);
+    hipLaunchKernelGGL((ns_tall_start_kernel<T, MUON>), dim3(wgs), dim3(T), p.lds, stream, p.tall, ios, st, h, ws);
+    CUTIE_CHECK_LAUNCH();
+    for (int k = 0; k < steps; ++k) {
+        hipLaunchKernelGGL((ns_tall_step_kernel<T, MUON>), dim3(wgs), dim3(T), p.lds, stream, p.tall, ios, st, h, k, (int)(k + 1 == steps),
+                           eps, ws);
         CUTIE_CHECK_LAUNCH();
     }
-    if (!p.ms.n) return CUTIE_OK;
-    for (int i = 0; i < p.ms.n; ++i) ios.io[i] = given.io[p.order[i]];
+    return CUTIE_OK;
+}
+
+template <bool MUON>
+inline int ns_run(const NsPlan& p, const Ios& ios, const Hyper& h, int steps, float eps, char* ws, hipStream_t stream) {
+    static_assert(sizeof(Mats) + sizeof(Ios) + sizeof(Starts) + sizeof(Hyper) + 64 < 4096, "kernel arguments");
+    static_assert(sizeof(Talls) + sizeof(Ios) + sizeof(Starts) + sizeof(Hyper) + 64 < 4096, "kernel arguments");
+    if (p.form == NsPlan::SMALL) {
+        CUTIE_ENSURE_LDS(ns_small_kernel<MUON>, p.lds);
+        hipLaunchKernelGGL((ns_small_kernel<MUON>), dim3((unsigned)p.sm.n), dim3(SMALL_THREADS), p.lds, stream, p.sm, ios, h, steps, eps);
+        CUTIE_CHECK_LAUNCH();
+        return CUTIE_OK;
+    }
     Starts st;
+    if (p.form == NsPlan::TALL) {
+        int wgs = 0;
+        for (int i = 0; i < p.tall.n; ++i) {
+            st.v[i] = wgs;
+            wgs += p.tall.t[i].tiles;
+        }
+        st.v[p.tall.n] = wgs;
+        // 16 waves where a workgroup has a CU to itself and its products are long enough for them (5634 x 42: 88 us, 8 waves 107;
+        // 32 of 7079 x 35: 430 us, 8 waves 343; 11 x 5496: 60, 8 waves 50)
+        return p.tall_wide && wgs <= 256 ? ns_tall<1024, MUON>(p, ios, st, h, wgs, steps, eps, ws, stream)
+                                         : ns_tall<512, MUON>(p, ios, st, h, wgs, steps, eps, ws, stream);
+    }
     const unsigned g0 = starts(p, st, [](const Mat& m, int) { return cdiv((int64_t)m.rows * m.cols, NORM_CHUNK); });
     hipLaunchKernelGGL((ns_norm_kernel<MUON>), dim3(g0), dim3(256), 0, stream, p.ms, ios, st, h, ws);
     CUTIE_CHECK_LAUNCH();

@@ -550,10 +550,10 @@ int cutie_opt_step(float* p, float* g, float* m, float* v, int64_t n, int64_t n_
  *     p_out may be its own p, m_out its own m; an output overlaps nothing else of the call.  S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq
  *     (nullable; the squared norm with S taken out, as cutie_opt_step leaves it) that is not finite or *invalid != 0 (nullable)
  *     makes p_out = p, m_out = m.
- * The products run on the matrix cores at f32 accuracy: operands are two f16 (22 bits), sums f32, sums of squares f64, all in
- * a fixed order: the same bits every run for one list of shapes (a matrix's bits depend on the others of its call: K is cut by their number).  X is kept to 2^-36 there: of a matrix whose norm lies
- * far below eps, less of the (then small) result is left.  A matrix of up to 64 x 192 values (either way round) is computed by one
- * workgroup in f32.
+ * The products run on the matrix cores at f32 accuracy: operands are two f16 (22 bits), sums f32, sums of squares f64, all in a
+ * fixed order: the same bits every run for one list of shapes (a matrix's bits depend on the others of its call: K is cut by
+ * their number).  X is kept to 2^-36 there: of a matrix whose norm lies far below eps, less of the (then small) result is left.
+ * Matrices of up to 64 values by 8192 (either way round) are computed in f32, small ones by one workgroup each.
  * Matrices are contiguous f32 [rows][cols], any size from 1 x 1 to 2^29 values (padded to multiples of 64), up to
  * CUTIE_MAX_BATCH a call, in one set of launches.  descs / shapes (rows, cols of each matrix) are HOST arrays.
  * workspace: cutie_orthogonalize_workspace_bytes(shapes, n) bytes for the same shapes in the same order, 256-byte aligned,

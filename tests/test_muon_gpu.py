@@ -376,3 +376,119 @@ def test_overlapping_outputs_are_refused():
             ops.muon_descs([(p, g, m, po, mo, 1.0)])
     ops.muon_descs([(p, g, m, p, m, 1.0)])
     ops.muon_descs([(p, g, m, w[24:48].view(4, 6), m, 1.0)])
+
+
+# sizes around the borders of the three forms: one workgroup, tiles of rows with S up to 64, the general one
+TALL = [(352, 16), (353, 16), (1, 353), (3, 400), (273, 32), (193, 48), (113, 64), (64, 129), (2049, 33), (17, 2050), (4100, 64), (8192, 5), (8193, 5)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "falling", "rank1", "one"])
+@pytest.mark.parametrize("r,c", TALL)
+def test_tall(r, c, kind):
+    g = torch.Generator().manual_seed(r + 7 * c)
+    u = matrix(r, c, kind, g)
+    want, tol = allowed(u)
+    buf = torch.full((r * c + 2,), 7.0, device=DEV)      # a misaligned matrix, and what lies around it
+    out = buf[1:-1].view(r, c)
+    ops.orthogonalize_batched([(u.to(DEV), out)])
+    assert float((out.cpu().double() - want).norm()) <= tol
+    assert float(buf[0]) == 7.0 and float(buf[-1]) == 7.0
+    out.copy_(u)
+    first = torch.empty(r, c, device=DEV)
+    ops.orthogonalize_batched([(out, first)])
+    ops.orthogonalize_batched([(out, out)])      # in place: the same bits
+    assert torch.equal(out, first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 6])
+@pytest.mark.parametrize("mag", [1e-25, 1.0, 1e37])
+def test_tall_steps_and_magnitudes(steps, mag):
+    """the tiles' parts are scaled by a power of two each: rows of very different sizes, tiles of zeros among them"""
+    g = torch.Generator().manual_seed(steps)
+    u = matrix(700, 20, "normal", g)
+    u[:64] *= 1e-20
+    u[128:192] = 0
+    u[300:] *= 1e-3
+    u = u * mag
+    for m in (u, u.t().contiguous()):
+        want, tol = allowed(m, steps, eps=1e-30)
+        out = torch.empty(m.shape, device=DEV)
+        ops.orthogonalize_batched([(m.to(DEV), out)], steps=steps, eps=1e-30)
+        assert float((out.cpu().double() - want).norm()) <= tol
+
+
+@pytest.mark.gpu
+def test_tall_zero_and_not_finite():
+    z, out = torch.zeros(900, 40, device=DEV), torch.full((900, 40), 7.0, device=DEV)
+    ops.orthogonalize_batched([(z, out)], eps=1e-38)
+    assert bool((out == 0).all())
+    good = torch.randn(50, 600, generator=torch.Generator().manual_seed(1))
+    bad = good.clone()
+    bad[3, 599] = float("nan")
+    inf = good.clone()
+    inf[49, 0] = float("-inf")
+    outs = [torch.empty(50, 600, device=DEV) for _ in range(3)]
+    ops.orthogonalize_batched([(t.to(DEV), o) for t, o in zip((bad, good, inf), outs)])
+    assert bool(torch.isnan(outs[0]).all()) and bool(torch.isnan(outs[2]).any())
+    want, tol = allowed(good)
+    assert float((outs[1].cpu().double() - want).norm()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 8, 9, 32])
+def test_tall_batches(n):
+    """up to 256 workgroups 64 columns are taken in tiles, from there on in the general form; 16 waves a workgroup or 8; small
+    and large matrices of the same call in between"""
+    g = torch.Generator().manual_seed(n)
+    shapes = [(2048, 64) if i % 4 != 3 else ((40, 2000), (300, 200), (20, 16))[i // 4 % 3] for i in range(n)]
+    us = [matrix(r, c, "normal", g) for r, c in shapes]
+    outs = [torch.empty(s, device=DEV) for s in shapes]
+    ops.orthogonalize_batched([(u.to(DEV), o) for u, o in zip(us, outs)])
+    for u, o in zip(us, outs):
+        want, tol = allowed(u)
+        assert float((o.cpu().double() - want).norm()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [None, 1024.0])
+def test_tall_muon_step_graph_and_skip(S):
+    gen = torch.Generator().manual_seed(8)
+    lr, mu, wd, l2, clip = 0.02, 0.95, 0.01, 5e-4, 0.5
+    shapes = [(3, 3, 64, 40), (30, 1000), (1027, 3)]
+    host = [tuple(torch.randn(sh, generator=gen) * s for s in (0.02, 1e-3 * (S or 1.0), 5e-3)) for sh in shapes]
+    ents = [[t.to(DEV) for t in h] for h in host]
+    gn = sum(((g / (S or 1.0)).double() ** 2).sum() for _, g, _ in host).float().reshape(1).to(DEV)
+    state = ops.loss_scale_state(S, DEV) if S else None
+    invalid = torch.zeros(1, dtype=torch.int32, device=DEV)
+    outs = [(torch.full_like(p, 7.0), torch.full_like(m, 7.0)) for p, _, m in ents]
+    plan = ops.muon_descs([(p, g, m, po, mo, 1.5) for (p, g, m), (po, mo) in zip(ents, outs)])
+    ws = torch.empty(ops.orthogonalize_workspace_bytes(plan[1]), dtype=torch.uint8, device=DEV)
+
+    def step():
+        ops.muon_step(plan, lr, momentum=mu, weight_decay=wd, l2=l2, gnorm_sq=gn, clip=clip, loss_scale=state, invalid=invalid, workspace=ws)
+    step()
+    gscale = clip / max(float(gn.double().sqrt()), clip)
+    for (p, g, m), (po, mo) in zip(host, outs):
+        u, m1, after = muon64(p, g / (S or 1.0), m, lr, mu, wd, l2, True, 1.5, gscale)
+        mag = mu * m.double().abs() + (g.double().abs() / (S or 1.0) + l2 * p.double().abs()) * gscale
+        assert bool(((mo.cpu().double() - m1).abs() <= 8 * U * mag).all())
+        x, off = allowed(u.reshape(-1, u.shape[-1]))
+        tol = lr * 1.5 * off + 4 * U * (float(p.double().norm()) + lr * 1.5 * float(x.norm()))
+        assert float((po.cpu().double() - after(x.reshape(p.shape))).norm()) <= tol
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for r in range(3):
+        for e in ents:
+            e[1].mul_(-0.7).add_(0.01)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for o in outs for t in o]
+        step()
+        assert all(torch.equal(a, b) for a, b in zip([t for o in outs for t in o], got)), r
+    invalid.fill_(1)
+    graph.replay()
+    for (p, _, m), (po, mo) in zip(ents, outs):
+        assert torch.equal(po, p) and torch.equal(mo, m)
