@@ -16,6 +16,10 @@
 // Layout.  L = max(rows, cols) rows of S = min(rows, cols) values, both padded with zeros to multiples of 64 (the transpose of
 // a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
 // of a product is one 128-byte line of a row.  A and B [S][S] alike.
+//
+// Measured (MI355X), five steps: 14 filters (11 of them 3840 x 256) 428 us, of which the matrix cores need 110 for the three
+// products at the rate of a large library product; 2048 x 8192 1.84 ms (1.45 ms likewise; in f32 the library's rate gives 3.6).
+// There are three forms: the general one of this comment, and two for fewer columns, in f32, below.
 #include "conv_common.h"
 
 namespace {
@@ -206,8 +210,8 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
 // 128-byte lines (hi and lo) go to LDS by buffer_load ... lds, STAGES of them, all but one in flight while that one is used.
 template <int F> struct Shape {
     static constexpr int T = 32 * F, HALF = T * 128, STAGE = 2 * HALF;      // bytes of one operand, of both
-    // F = 4: two workgroups a CU with two stages (14 filters 475 us, 2048 x 8192 1.82 ms) beat one with three or four (558, 567 us;
-    // 2.28, 2.25 ms).  F = 2: three stages 475 us, two 480, four 475.
+    // F = 4: two workgroups a CU with two stages (14 filters 458 us, 2048 x 8192 1.84 ms) beat one with three (535 us, 2.29 ms).
+    // F = 2: two, three and four stages are alike.
     static constexpr int STAGES = F == 4 ? 2 : 3;
     static constexpr int LDS = STAGES * STAGE;
     static constexpr int PIECES = T / 8;      // 1-KB pieces of an operand; a wave moves PIECES / 4 of each
@@ -861,7 +865,7 @@ __global__ __launch_bounds__(T) void ns_tall_step_kernel(Talls ts, Ios ios, Star
 
 // ------------------------------------------------------------------------------------------------------------------- host
 // All matrices of a call are computed in one form, the cheapest that takes every one of them: a matrix more in a form's launches costs
-// little, the launches of a second form come on top (14 filters of which one is 7680 x 64 and one 64 x 18: 475 us with those two in
+// little, the launches of a second form come on top (14 filters of which one is 7680 x 64 and one 64 x 18: 458 us; with those two in
 // launches of their own forms 575).
 struct NsPlan {
     enum { SMALL, TALL, GENERAL } form;
@@ -946,8 +950,10 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
         m.Lp = (int)Lp;
         m.Sp = (int)Sp;
     }
-    // The 128 tile where it gives every CU a workgroup, K cut into pieces of eight steps where it can be (14 filters: 475 us; with
-    // the 64 tile for X B 526, for X^T X 532); two workgroups a CU by cutting K (512 / tiles: 475 us, 256 530, 1024 538)
+    // X B and A A: the 128 tile where it gives every CU a workgroup (A A: with K cut into pieces of eight steps; 14 filters 458 us,
+    // with the 64 tile for X B 486; 2048 x 8192 1.84 ms, 2.49).  X^T X: where it gives each four (2048 x 8192 1.84 ms, 64 tile 2.14;
+    // 32 of 3840 x 256 832 us, 898), else the 64 tile, which wastes less of the diagonal's tiles (14 filters 428 us, 128 tile 458;
+    // two of 4608 x 512 306, 345).  K is cut for two workgroups a CU (512 / tiles; 256 / tiles 2.25 ms, 1024 / tiles for 14 filters 496 us)
     int64_t tg = 0, ts = 0, ta = 0;
     for (int i = 0; i < n; ++i) {
         const Mat& m = p.ms.m[i];
@@ -955,7 +961,7 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
         ts += (int64_t)tri_tiles(m.Sp, 4) * cdiv(m.Sp, 256);
         ta += cdiv(m.Lp, 128) * cdiv(m.Sp, 128);
     }
-    p.fg = tg >= 256 ? 4 : 2;
+    p.fg = tg >= 1024 ? 4 : 2;
     p.fs = ts >= 256 ? 4 : 2;
     p.fa = ta >= 256 ? 4 : 2;
     int64_t ng = 0, nq = 0;
