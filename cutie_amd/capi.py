@@ -222,6 +222,8 @@ def ld_of(t):
     for d in range(len(strides) - 2):
         if strides[d] != strides[d + 1] * shape[d + 1]:
             raise CutieError("view is not row-collapsible: shape %s strides %s" % (tuple(shape), strides))
+    if strides[-2] > 0x7fffffff:      # an int in the C ABI
+        raise CutieError("leading dimension %d is beyond 2^31 - 1" % strides[-2])
     return strides[-2]
 
 

@@ -713,10 +713,21 @@ inline GnSpace gn_space(int B, int HW, int C, int G) {
     return w;
 }
 
+// whether [rows][ld] views of C columns share an element: slices of one wide buffer do not
+inline bool gn_overlap(const void* a, int ld_a, const void* b, int ld_b, int64_t rows, int C, int es) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t na = (uintptr_t)((rows - 1) * ld_a + C) * es, nb = (uintptr_t)((rows - 1) * ld_b + C) * es;
+    if (x >= y + nb || y >= x + na) return false;
+    if (ld_a != ld_b) return true;
+    const uintptr_t row = (uintptr_t)ld_a * es, d = (x > y ? x - y : y - x) % row;
+    return d < (uintptr_t)C * es || row - d < (uintptr_t)C * es;
+}
+
 inline int gn_check(const char* who, int B, int HW, int C, int G, int act, int dt) {
     CUTIE_CHECK_ARG(B >= 0 && HW >= 0 && C >= 1 && G >= 1 && C % G == 0, "%s: B=%d HW=%d C=%d groups=%d (groups must divide C)", who, B,
                     HW, C, G);
     CUTIE_CHECK_ARG(B <= 65535 && G <= 65535 && C <= 65535, "%s: B=%d, groups=%d, C=%d (at most 65535 each)", who, B, G, C);
+    CUTIE_CHECK_ARG(HW <= (1 << 30), "%s: HW=%d (at most 2^30)", who, HW);
     CUTIE_CHECK_ARG(act >= GN_ACT_NONE && act <= GN_ACT_SILU, "%s: activation code %d (0 none, 1 ReLU, 2 sigmoid, 3 SiLU)", who, act);
     CUTIE_CHECK_ARG(dt == CUTIE_F32 || dt == CUTIE_BF16 || dt == CUTIE_F16, "%s: unknown dtype %d", who, dt);
     return CUTIE_OK;
@@ -744,7 +755,9 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
     const int lds[2] = {ld_x, ld_y};
     const int vec = gn_vec(dtype, C / groups, ptrs, lds, 2);
     const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX, 1024);
+    const bool lap = gn_overlap(x, ld_x, y, ld_y, (int64_t)B * HW, C, elem_bytes(dtype));
     if (p.resident) {
+        CUTIE_CHECK_ARG(!lap, "gn_fwd: y overlaps x");
         const dim3 grid((unsigned)(cdiv(p.s.items, 8) * 8));
         CUTIE_DISPATCH_DTYPE(dtype, DT, {
             typedef typename elem<DT>::type E;
@@ -766,6 +779,7 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
         set_error("gn_fwd: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
         return CUTIE_E_WORKSPACE;
     }
+    CUTIE_CHECK_ARG(!lap, "gn_fwd: y overlaps x");
     char* ws = (char*)workspace;
     double* slots = (double*)(ws + w.slots);
     float* low = (float*)(ws + w.low);
@@ -803,6 +817,8 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
         set_error("gn_bwd: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
         return CUTIE_E_WORKSPACE;
     }
+    CUTIE_CHECK_ARG(none || !(gn_overlap(dy, ld_dy, dx, ld_dx, (int64_t)B * HW, C, es) || gn_overlap(x, ld_x, dx, ld_dx, (int64_t)B * HW, C, es)),
+                    "gn_bwd: dx overlaps dy or x");
     char* ws = (char*)workspace;
     float* chan = ws ? (float*)(ws + w.chan) : nullptr;
     if (!none) {

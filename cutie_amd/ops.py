@@ -81,6 +81,8 @@ def _rows_ld(t):
 
 def _check_ids(what, ids, rows, table):
     V, E = table.shape
+    if V >= 1 << 30 or E > 65536:      # ints in the C ABI, whose own check would see them cut off
+        raise capi.CutieError("%s: a table of %d x %d (below 2^30 rows of at most 65536)" % (what, V, E))
     if ids.dtype != torch.int32 or not ids.is_contiguous():
         raise capi.CutieError("%s: ids must be contiguous int32" % what)
     if table.dtype != torch.float32 or not table.is_contiguous():
@@ -455,7 +457,10 @@ def _gn_views(what, x, stats, act, others):
     for t in others:
         if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
             raise capi.CutieError("%s: views differ: %s %s against %s %s" % (what, tuple(t.shape), t.dtype, tuple(x.shape), x.dtype))
-    return _bhwc(x)
+    B, HW, C = _bhwc(x)
+    if HW > 1 << 30 or max(B, C) > 65535:      # ints in the C ABI
+        raise capi.CutieError("%s: B=%d, H*W=%d, C=%d (at most 65535, 2^30, 65535)" % (what, B, HW, C))
+    return B, HW, C
 
 
 def _gn_ld(t):
@@ -662,6 +667,8 @@ def _matrix(t, what, like=None):
         raise capi.CutieError("%s: tensors differ: %s on %s against %s on %s" % (what, tuple(t.shape), t.device, tuple(like.shape), like.device))
     if t.numel() == 0:
         raise capi.CutieError("%s: an empty matrix" % what)
+    if t.numel() > 1 << 29:
+        raise capi.CutieError("%s: a matrix of %d values (at most 2^29)" % (what, t.numel()))
     return t.numel() // t.shape[-1], t.shape[-1]
 
 
@@ -735,9 +742,10 @@ def muon_step(entries, lr, momentum=0.95, nesterov=True, weight_decay=0.0, l2=0.
     orthogonalize_workspace_bytes(shapes) bytes."""
     arr, shapes, device = entries if isinstance(entries, tuple) else muon_descs(entries)
     ws = _orth_space(shapes, device, workspace, "muon_step")
-    for t, what, dt in ((gnorm_sq, "gnorm_sq", torch.float32), (loss_scale, "loss_scale", torch.float32), (invalid, "invalid", torch.int32)):
-        if t is not None and (t.dtype != dt or t.device != device):
-            raise capi.CutieError("muon_step: %s must be %s on %s" % (what, dt, device))
+    for t, what, dt, n in ((gnorm_sq, "gnorm_sq", torch.float32, 1), (loss_scale, "loss_scale", torch.float32, 2),
+                           (invalid, "invalid", torch.int32, 1)):
+        if t is not None and (t.dtype != dt or t.device != device or t.numel() < n or not t.is_contiguous()):
+            raise capi.CutieError("muon_step: %s must be contiguous %s of at least %d on %s" % (what, dt, n, device))
     call("cutie_muon_step", arr, len(arr), float(lr), float(momentum), 1 if nesterov else 0, float(weight_decay), float(l2), int(steps),
          float(eps), ptr(gnorm_sq), float(clip), float(grad_scale), ptr(loss_scale), ptr(invalid), ptr(ws),
          ws.numel() * ws.element_size(), stream(device))

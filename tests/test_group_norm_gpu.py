@@ -371,3 +371,48 @@ def test_workspace_size():
     n = capi.lib().cutie_gn_workspace_bytes
     assert n(1, 4, 8, 3) == 0 and n(0, 4, 8, 2) == 0
     assert n(32, 4096, 256, 32) >= 32 * 256 * 8
+
+
+@pytest.mark.parametrize("y,ld_x,ld_y", [(4096 + 4, 64, 64), (4096 + 28, 64, 64), (4096 + 64 * 4 - 28, 64, 64), (4096 + 3 * 64 * 4, 64, 64),
+                                         (4096 - 64 * 4 + 4, 64, 64), (4096 + 32, 64, 128)])
+@pytest.mark.parametrize("HW", [4, 1 << 20])
+def test_overlapping_views_are_refused(y, ld_x, ld_y, HW):
+    """rows of 8 f32 channels: refused on the host, nothing is launched"""
+    v = ctypes.c_void_p
+    ws, n = v(1 << 40), 1 << 40
+    assert fwd_rc(y=v(y), ld_x=ld_x, ld_y=ld_y, HW=HW, ws=ws, n=n) == -1 and b"overlaps" in capi.lib().cutie_last_error()
+    for dy, x in ((4096, 1 << 36), (1 << 36, 4096)):
+        rc = capi.lib().cutie_gn_bwd(v(dy), ld_x, v(x), ld_x, None, None, 2, 0, v(1 << 41), v(y), ld_y, 0, None, None, 0, 1, HW, 8, ws, n, None)
+        assert rc == -1 and b"overlaps" in capi.lib().cutie_last_error()
+
+
+def test_sizes_beyond_the_c_abi_are_refused():
+    for shape in ((1, 1 << 16, 1 << 16, 1), (65536, 1, 1, 1), (1, 1, 1, 65536)):
+        x = torch.empty(shape, device="meta")
+        with pytest.raises(capi.CutieError, match="at most"):
+            ops.gn_fwd(x, x, torch.empty(shape[0], 1, 2, device="meta"))
+    x = torch.empty_strided((1, 1, 2, 1), (1 << 33, 1 << 33, 1 << 32, 1), device="meta")
+    with pytest.raises(capi.CutieError, match="leading dimension"):
+        capi.ld_of(x)
+    with pytest.raises(capi.CutieError, match="below 2"):
+        ops._check_ids("embed_grad_sorted", torch.empty(3, dtype=torch.int32, device="meta"), torch.empty(3, 1, device="meta"),
+                       torch.empty((1 << 32) + 3, 1, device="meta"))
+
+
+@pytest.mark.gpu
+def test_slices_of_one_buffer_are_taken():
+    """x, y and the gradients as neighbouring channel slices"""
+    g = torch.Generator().manual_seed(4)
+    wide = torch.randn(2, 5, 7, 48, generator=g).to(DEV)
+    xs = wide[..., 8:16].clone()
+    st, st2 = torch.empty(2, 2, 2, device=DEV), torch.empty(2, 2, 2, device=DEV)
+    want = torch.empty(2, 5, 7, 8, device=DEV)
+    ops.gn_fwd(xs, want, st, act="silu")
+    ops.gn_fwd(wide[..., 8:16], wide[..., 16:24], st2, act="silu")
+    assert torch.equal(wide[..., 16:24], want) and torch.equal(st, st2)
+    dy = wide[..., 24:32].clone()
+    ops.gn_bwd(dy, xs, st, want, act="silu")
+    ops.gn_bwd(wide[..., 24:32], wide[..., 8:16], st, wide[..., 0:8], act="silu")
+    assert torch.equal(wide[..., 0:8], want)
+    with pytest.raises(capi.CutieError, match="overlaps"):
+        ops.gn_fwd(wide[..., 8:16], wide[..., 12:20], st2)

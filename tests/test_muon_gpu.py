@@ -492,3 +492,55 @@ def test_tall_muon_step_graph_and_skip(S):
     graph.replay()
     for (p, _, m), (po, mo) in zip(ents, outs):
         assert torch.equal(po, p) and torch.equal(mo, m)
+
+
+def test_call_overlaps_are_refused():
+    """the same matrix twice, an output over another matrix's tensors: refused on the host, nothing is launched"""
+    lib = capi.lib()
+
+    def orth(*pairs):
+        d = (capi.OrthDesc * len(pairs))()
+        for x, (g, out) in zip(d, pairs):
+            x.g, x.out, x.rows, x.cols = g, out, 16, 16      # 1024 bytes each
+        rc = lib.cutie_orthogonalize_batched(d, len(pairs), 5, 1e-7, P(1 << 20), 1 << 40, None)
+        return rc, lib.cutie_last_error()
+    for pairs in (((4096, 4096), (4096, 4096)), ((4096, 8192), (8192, 16384)), ((4096, 8192), (12288, 8192)), ((4096, 4100),),
+                  ((4096, 5116),), ((4096, 8192), (12288, 9212))):
+        rc, err = orth(*pairs)
+        assert rc == -1 and b"overlaps" in err, pairs
+
+    def muon(*mats):
+        d = (capi.MuonDesc * len(mats))()
+        for x, t in zip(d, mats):
+            x.p, x.g, x.m, x.p_out, x.m_out = (1024 * k for k in t)
+            x.rows, x.cols, x.out_scale = 16, 16, 1.0
+        rc = lib.cutie_muon_step(d, len(mats), 0.1, 0.9, 1, 0.0, 0.0, 5, 1e-7, None, 0.0, 1.0, None, None, P(1 << 20), 1 << 40, None)
+        return rc, lib.cutie_last_error()
+    for mats in (((1, 2, 3, 1, 3), (1, 4, 5, 1, 5)), ((1, 2, 3, 4, 5), (6, 4, 7, 6, 7)), ((1, 2, 3, 3, 1),), ((1, 2, 3, 4, 4),),
+                 ((1, 2, 3, 2, 3),), ((1, 2, 3, 1, 3), (4, 5, 3, 4, 6))):
+        rc, err = muon(*mats)
+        assert rc == -1 and b"overlaps" in err, mats
+
+
+def test_sizes_beyond_the_c_abi_are_refused():
+    meta = torch.empty(((1 << 32) + 5, 1), device="meta")
+    with pytest.raises(capi.CutieError, match="2\\^29"):
+        ops.orthogonalize_batched([(meta, meta)])
+    w = torch.zeros(4, 6)
+    plan = (None, [(4, 6)], w.device)
+    for kw in (dict(loss_scale=torch.zeros(1)), dict(gnorm_sq=torch.zeros(0)), dict(invalid=torch.zeros(1)), dict(gnorm_sq=torch.zeros(1).half())):
+        with pytest.raises(capi.CutieError, match="must be"):
+            ops.muon_step(plan, 0.1, **kw)
+
+
+@pytest.mark.gpu
+def test_shared_inputs_and_neighbours_are_taken():
+    g = torch.randn(64, 16, generator=torch.Generator().manual_seed(1)).to(DEV)
+    w = torch.empty(2 * g.numel(), device=DEV)
+    a, b = w[:g.numel()].view(64, 16), w[g.numel():].view(64, 16)
+    ops.orthogonalize_batched([(g, a), (g, b)])      # one input twice, outputs side by side
+    assert torch.equal(a, b)
+    want, tol = allowed(g.cpu())
+    assert float((a.cpu().double() - want).norm()) <= tol
+    with pytest.raises(capi.CutieError, match="overlaps"):
+        ops.orthogonalize_batched([(g, a), (g, a)])
