@@ -113,14 +113,15 @@ __device__ __forceinline__ void store4(bf16_t* p, float4 v) {
 template <int DT, int VEC> struct Pack {
     typedef typename elem<DT>::type T;
     typedef T V __attribute__((ext_vector_type(VEC)));
+    typedef V U __attribute__((aligned(sizeof(T))));      // in memory: the hardware loads a vector from any element's address
     V v;
-    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const U*>(p); }
     __device__ __forceinline__ float get(int e) const { T t = v[e]; return load_as_f32(&t); }
     __device__ __forceinline__ void set(int e, float f) { T t; store_from_f32(&t, f); v[e] = t; }
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<U*>(p) = v; }
     // non-temporal: for a tensor that is touched once and larger than the caches
-    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p)); }
-    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
+    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const U*>(p)); }
+    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<U*>(p)); }
 };
 template <int DT> struct Pack<DT, 1> {
     typedef typename elem<DT>::type T;

@@ -8,12 +8,13 @@
 // Both directions are HBM-bound: 2 (forward) or 3 (backward) tensors moved, ~12 / ~25 operations an element.
 //
 // Two forms.  RESIDENT: a workgroup owns whole groups of one sample and keeps their values in registers (and LDS) between the
-// sums and the store, so each tensor is moved once.  SPLIT, where a group does not fit a workgroup: per-channel sums over
-// slices of HW, a small fold, and a second pass over the operands.
+// sums and the store, so each tensor is moved once.  SPLIT, where a group does not fit a workgroup, or where the pieces of a
+// pixel are so narrow or the groups so few that it takes longer (gn_resident_us): per-channel sums over slices of HW, a small
+// fold, and a second pass over the operands.
 //
 // Measured (MI355X), 32 x 64 x 64 x 256, 32 groups (134 MB forward, 201 MB backward), inputs that change from call to call: forward
 // f16 33 us resident (4.1 TB/s), backward bf16 SiLU 73 us + 5 us fold (2.6 TB/s).  The same inputs again, partly in cache: 30 and
-// 54 + 5 us; split form 52 and 95.  What decides is the width of the piece of a pixel that a workgroup reads (its groups'
+// 54 + 5 us; split form 50 and 86.  What decides is the width of the piece of a pixel that a workgroup reads (its groups'
 // channels): 16 bytes 50 us forward, 32 bytes 31, 64 bytes 30 - L2 hands out 64 bytes at least - and, backward, one exponential
 // and one reciprocal an element instead of two (86 us when the store pass made g again).  Non-temporal stores: 38 and 90 us
 // (pieces of a line no longer meet in L2).  The backward keeps 128 KB of x in LDS, so a CU holds one workgroup and its loads wait
@@ -449,9 +450,10 @@ __global__ __launch_bounds__(256) void gn_fwd_fold(const double* __restrict__ sl
     const int Cg = C / G, g = blockIdx.x;
     const int64_t b = blockIdx.y;
     double a = 0, q = 0;
-    const int64_t n = (int64_t)T * Cg;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-        const int64_t t = i / Cg;
+    const unsigned n = (unsigned)T * Cg;      // T <= 256
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < n; i += 256) {
+        const unsigned t = i / (unsigned)Cg;
         const double2 v = *reinterpret_cast<const double2*>(slots + ((b * T + t) * C + g * Cg + (i - t * Cg)) * 2);
         a += v.x;
         q += v.y;
@@ -484,9 +486,11 @@ __global__ __launch_bounds__(256) void gn_fwd_apply(const typename elem<DT>::typ
     if (!m.on) return;
     const int Cg = C / G;
     float mean[VEC], rg[VEC], be[VEC];
+    int run = m.c0 / Cg;      // the group of channel c0 + e: at most one further with every channel
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const int64_t g = m.b * G + (m.c0 + e) / Cg;
+        run += m.c0 + e == (run + 1) * Cg;
+        const int64_t g = m.b * G + run;
         mean[e] = stats[g * 2];
         rg[e] = stats[g * 2 + 1] * (gamma ? gamma[m.c0 + e] : 1.f);
         be[e] = fmaf(-low[g], rg[e], beta ? beta[m.c0 + e] : 0.f);
@@ -506,9 +510,11 @@ __global__ __launch_bounds__(256) void gn_fwd_apply(const typename elem<DT>::typ
 template <int VEC>
 __device__ __forceinline__ void norms(Norm1* ch, const SplitMap<VEC>& m, int Cg, int G, const float* stats, const float* gamma,
                                       const float* beta) {
+    int run = m.c0 / Cg;      // the group of channel c0 + e: at most one further with every channel
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const int64_t g = m.b * G + (m.c0 + e) / Cg;
+        run += m.c0 + e == (run + 1) * Cg;
+        const int64_t g = m.b * G + run;
         ch[e].mean = stats[g * 2];
         ch[e].rstd = stats[g * 2 + 1];
         ch[e].beta = beta ? beta[m.c0 + e] : 0.f;
@@ -558,20 +564,31 @@ __global__ __launch_bounds__(256) void gn_bwd_fold(const float* __restrict__ slo
     const int Cg = C / G, g = blockIdx.x;
     const int64_t b = blockIdx.y;
     float h0 = 0.f, h1 = 0.f;
-    for (int c = threadIdx.x; c < Cg; c += 256) {
-        const int cc = g * Cg + c;
+    // `parts` threads a channel take every parts-th slot, their sums are added in order
+    const int w = min(Cg, 256), parts = 256 / w, col = threadIdx.x % w, part = threadIdx.x / w;
+    for (int c0 = 0; c0 < Cg; c0 += w) {
+        const int c = c0 + col, cc = g * Cg + c;
         float a = 0.f, q = 0.f;
+        if (part < parts && c < Cg) {
 #pragma unroll 8
-        for (int t = 0; t < T; ++t) {
-            const float2 v = *reinterpret_cast<const float2*>(slots + ((b * T + t) * C + cc) * 2);
-            a += v.x;
-            q += v.y;
+            for (int t = part; t < T; t += parts) {
+                const float2 v = *reinterpret_cast<const float2*>(slots + ((b * T + t) * C + cc) * 2);
+                a += v.x;
+                q += v.y;
+            }
         }
-        chan[(b * C + cc) * 2] = a;
-        chan[(b * C + cc) * 2 + 1] = q;
-        const float ga = gamma ? gamma[cc] : 1.f;
-        h1 = fmaf(a, ga, h1);
-        h0 = fmaf(q, ga, h0);
+        red[0][threadIdx.x] = a;
+        red[1][threadIdx.x] = q;
+        __syncthreads();
+        if (part == 0 && c < Cg) {
+            for (int k = 1; k < parts; ++k) { a += red[0][k * w + col]; q += red[1][k * w + col]; }
+            chan[(b * C + cc) * 2] = a;
+            chan[(b * C + cc) * 2 + 1] = q;
+            const float ga = gamma ? gamma[cc] : 1.f;
+            h1 = fmaf(a, ga, h1);
+            h0 = fmaf(q, ga, h0);
+        }
+        __syncthreads();
     }
     red[0][threadIdx.x] = h0;
     red[1][threadIdx.x] = h1;
@@ -601,9 +618,11 @@ __global__ __launch_bounds__(256) void gn_bwd_apply(const typename elem<DT>::typ
     Norm1 ch[VEC];
     float s0[VEC], s1[VEC];
     norms<VEC>(ch, m, Cg, G, stats, gamma, beta);
+    int run = m.c0 / Cg;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const int64_t g = m.b * G + (m.c0 + e) / Cg;
+        run += m.c0 + e == (run + 1) * Cg;
+        const int64_t g = m.b * G + run;
         s0[e] = grp[g * 2] * ch[e].rstd;
         s1[e] = grp[g * 2 + 1] * ch[e].rstd * ch[e].rstd;
     }
@@ -625,36 +644,57 @@ __global__ __launch_bounds__(256) void gn_bwd_apply(const typename elem<DT>::typ
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
+constexpr int SLICE = 8192, ROWS = 8;      // of the split form's two passes (8 x 128 x 128 x 64 f16 backward: 29 us; 4 rows 33)
 inline int elem_bytes(int dt) { return dt == CUTIE_F32 ? 4 : 2; }
 
-// slices of HW a sample is cut into in the split form: enough workgroups for the chip, at least 32 pixels each
+// slices of HW that a sample is cut into for the sums of the split form: enough workgroups for the chip, but at least 32 pixels
+// and SLICE values each
 inline int gn_slices(int B, int HW, int C) {
     int64_t t = cdiv(2048, (int64_t)B * cdiv(C, 1024));
-    const int64_t most = cdiv(HW, 32);
+    int64_t most = cdiv(HW, 32);
+    if (most > cdiv((int64_t)HW * C, SLICE)) most = cdiv((int64_t)HW * C, SLICE);
     if (t > most) t = most;
     if (t > 256) t = 256;
     return t < 1 ? 1 : (int)t;
 }
+// and for its second pass, whose slices leave nothing behind: ROWS pixels a thread
+inline unsigned gn_apply_slices(int HW, int C, int vec) {
+    const int cv = C / vec;
+    const int64_t t = cdiv(HW, (int64_t)(256 / (cv < 256 ? cv : 256)) * ROWS);
+    return (unsigned)(t > 65535 ? 65535 : t);
+}
 
-// The widest vector that all views allow: base addresses and row strides must be multiples of it, and it must divide
-// `run`, the number of consecutive channels it may not cross.
-inline int gn_vec(int dt, int run, const void* const* ptrs, const int* lds, int n) {
-    const int es = elem_bytes(dt);
-    for (int v = 16 / es; v > 1; v >>= 1) {
-        if (v == 2 && es == 2) break;       // 4-byte vectors are not built: 16, 8 (16-bit types) bytes, or single elements
-        if (v == 2 && es == 4) break;
-        bool ok = run % v == 0;
-        for (int i = 0; i < n && ok; ++i)
-            ok = (reinterpret_cast<uintptr_t>(ptrs[i]) % (uintptr_t)(v * es)) == 0 && lds[i] % v == 0;
-        if (ok) return v;
-    }
-    return 1;
+// Values of a vector: as many of `run` consecutive channels as 16 bytes hold, wherever a row begins (32 x 64 x 64 x 256 f16 in rows of
+// 257: 47 us forward, single elements 68)
+inline int gn_vec(int dt, int run) {
+    if (dt == CUTIE_F32) return run % 4 == 0 ? 4 : 1;
+    return run % 8 == 0 ? 8 : (run % 4 == 0 ? 4 : 1);
+}
+
+// of the split form, whose threads carry their channels' constants: four (8 x 128 x 128 x 64 f16 29 us backward, eight 35, single elements
+// 32), eight of a wide row (512 x 512 x 1024: 622 us, four 713)
+inline int gn_split_vec(int dt, int C) {
+    const int v = gn_vec(dt, C);
+    return v == 8 && C < 1024 ? 4 : v;
 }
 
 struct GnPlan { bool resident; int threads, K; GnShape s; };
 
+// What the two forms take, roughly, in us: the resident form by rounds of workgroups (a forward CU holds two of them, a backward CU
+// one) and the lines that a workgroup touches - pieces of a pixel below 64 bytes move 64 all the same - the split form by its
+// launches and the bytes of a tensor.  Resident / split, measured: 8 x 64 x 64 x 66 f16, 33 groups 15 / 18 forward and 24 / 27 backward,
+// 16 of them 26 / 19 and 37 / 31; 32 x 64 x 64 x 256 f16, 128 groups 117 / 54 and 173 / 92, 32 groups 31 / 50 and 76 / 86;
+// 4 x 128 x 128 x 64 f16, 8 groups 36 / 18 forward; 8 x 128 x 128 x 256 f16, 32 groups 65 / 50 forward; 8 x 64 x 64 x 264 f16, 33 groups 20 / 22 and 44 / 33; 32 x 64 x 64 x 24, 3 groups 12 / 18
+// and 19 / 24.
+inline double gn_resident_us(const GnShape& s, int es, bool bwd) {
+    const double piece = (double)s.gc * s.Cg * es, rounds = (double)s.items / 256;
+    if (bwd) return cdiv(s.items, 256) * (9.0 + 0.75 * piece) * s.HW / 4096;
+    return 3.0 + (rounds < 1 ? 1 : rounds) * s.HW * (piece < 64 ? 64 : piece) / 25e3;
+}
+inline double gn_split_us(int64_t bytes, bool bwd) { return bwd ? 22 + bytes * 1e-6 : 13 + bytes * 0.45e-6; }
+
 // kmax: vectors of `vec` elements a thread may hold; tmax: threads of a workgroup
-inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax, int tmax) {
+inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax, int tmax, bool bwd) {
     GnPlan p = {};
     const int Cg = C / G, es = elem_bytes(dt);
     p.s.HW = HW; p.s.C = C; p.s.G = G; p.s.Cg = Cg;
@@ -683,7 +723,7 @@ inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax, in
     p.K = (int)cdiv(HW, p.s.rows_par);
     auto pow2 = [](int64_t v) { return v <= 64 && (v & (v - 1)) == 0; };
     p.s.fast = pow2(cv) && pow2(cv / gc);
-    p.resident = p.K <= kmax && p.s.items <= (1 << 30);
+    p.resident = p.K <= kmax && p.s.items <= (1 << 30) && gn_resident_us(p.s, es, bwd) <= gn_split_us((int64_t)B * HW * C * es, bwd);
     return p;
 }
 
@@ -751,10 +791,8 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
     CUTIE_CHECK_ARG(x != y, "gn_fwd: y must not be x");
     CUTIE_CHECK_ARG(reinterpret_cast<uintptr_t>(x) % elem_bytes(dtype) == 0 && reinterpret_cast<uintptr_t>(y) % elem_bytes(dtype) == 0,
                     "gn_fwd: misaligned pointers");
-    const void* ptrs[2] = {x, y};
-    const int lds[2] = {ld_x, ld_y};
-    const int vec = gn_vec(dtype, C / groups, ptrs, lds, 2);
-    const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX, 1024);
+    const int vec = gn_vec(dtype, C / groups);
+    const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX, 1024, false);
     const bool lap = gn_overlap(x, ld_x, y, ld_y, (int64_t)B * HW, C, elem_bytes(dtype));
     if (p.resident) {
         CUTIE_CHECK_ARG(!lap, "gn_fwd: y overlaps x");
@@ -783,15 +821,15 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
     char* ws = (char*)workspace;
     double* slots = (double*)(ws + w.slots);
     float* low = (float*)(ws + w.low);
-    const int sv = gn_vec(dtype, C, ptrs, lds, 2), T = gn_slices(B, HW, C);
-    const dim3 grid((unsigned)T, (unsigned)B, (unsigned)cdiv(C / sv, 256));
+    const int sv = gn_split_vec(dtype, C), T = gn_slices(B, HW, C);
+    const dim3 grid((unsigned)T, (unsigned)B, (unsigned)cdiv(C / sv, 256)), apply(gn_apply_slices(HW, C, sv), grid.y, grid.z);
     CUTIE_DISPATCH_DTYPE(dtype, DT, {
         typedef typename elem<DT>::type E;
         GN_VECS(DT, sv, VEC, {
             hipLaunchKernelGGL((gn_fwd_partial<DT, VEC>), grid, dim3(256), 0, stream, (const E*)x, ld_x, HW, C, slots);
             hipLaunchKernelGGL(gn_fwd_fold, dim3((unsigned)groups, (unsigned)B), dim3(256), 0, stream, slots, T, HW, C, groups, eps, stats,
                                low);
-            hipLaunchKernelGGL((gn_fwd_apply<DT, VEC>), grid, dim3(256), 0, stream, (const E*)x, ld_x, gamma, beta, stats, low, act, (E*)y,
+            hipLaunchKernelGGL((gn_fwd_apply<DT, VEC>), apply, dim3(256), 0, stream, (const E*)x, ld_x, gamma, beta, stats, low, act, (E*)y,
                                ld_y, HW, C, groups);
         })
     });
@@ -822,10 +860,8 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
     char* ws = (char*)workspace;
     float* chan = ws ? (float*)(ws + w.chan) : nullptr;
     if (!none) {
-        const void* ptrs[3] = {dy, x, dx};
-        const int lds[3] = {ld_dy, ld_x, ld_dx};
-        const int vec = gn_vec(dtype, C / groups, ptrs, lds, 3);
-        const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, vec > 1 ? 16 : 24, vec > 1 ? 512 : 1024);
+        const int vec = gn_vec(dtype, C / groups);
+        const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, vec > 1 ? 16 : 24, vec > 1 ? 512 : 1024, true);
         if (p.resident) {
             const dim3 grid((unsigned)(cdiv(p.s.items, 8) * 8));
             const size_t sums = params ? (size_t)2 * p.threads * vec * sizeof(float) : 0;
@@ -855,8 +891,8 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
         } else {
             float* slots = (float*)(ws + w.slots);
             float* grp = (float*)(ws + w.grp);
-            const int sv = gn_vec(dtype, C, ptrs, lds, 3), T = gn_slices(B, HW, C);
-            const dim3 grid((unsigned)T, (unsigned)B, (unsigned)cdiv(C / sv, 256));
+            const int sv = gn_split_vec(dtype, C), T = gn_slices(B, HW, C);
+            const dim3 grid((unsigned)T, (unsigned)B, (unsigned)cdiv(C / sv, 256)), apply(gn_apply_slices(HW, C, sv), grid.y, grid.z);
             CUTIE_DISPATCH_DTYPE(dtype, DT, {
                 typedef typename elem<DT>::type E;
                 GN_VECS(DT, sv, VEC, {
@@ -864,7 +900,7 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
                                        beta, stats, act, HW, C, groups, slots);
                     hipLaunchKernelGGL(gn_bwd_fold, dim3((unsigned)groups, (unsigned)B), dim3(256), 0, stream, slots, T, HW, C, groups,
                                        gamma, chan, grp);
-                    hipLaunchKernelGGL((gn_bwd_apply<DT, VEC>), grid, dim3(256), 0, stream, (const E*)dy, ld_dy, (const E*)x, ld_x, gamma,
+                    hipLaunchKernelGGL((gn_bwd_apply<DT, VEC>), apply, dim3(256), 0, stream, (const E*)dy, ld_dy, (const E*)x, ld_x, gamma,
                                        beta, stats, grp, act, (E*)dx, ld_dx, HW, C, groups);
                 })
             });

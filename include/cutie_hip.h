@@ -358,7 +358,7 @@ int cutie_spatial_mean_bcast(const void* x, int ld_x, int x_dtype, void* out, in
  *        dx = rstd * (g*gamma - mean_N(g*gamma) - xhat * mean_N(g*gamma*xhat)),
  *        dgamma[c] = sum g * xhat, dbeta[c] = sum g over (b, hw)  (each nullable; accumulate != 0 adds to what is there)
  * gamma / beta f32 [C], each nullable (1 and 0).  x, y, dy, dx share one dtype, any channel count that `groups` divides, any
- * leading dimension >= C; views whose base, leading dimension and group width are multiples of 16 bytes move fastest.
+ * leading dimension >= C; groups of 16 bytes or a multiple of them move fastest, in views whose base and leading dimension are such.
  * An output may not overlap an input (slices of one wide buffer are fine).  Sums are f32 or f64 in a fixed order: reruns are bit-identical.  A value next to the
  * step of the ReLU takes the side that f64 arithmetic on (x, stats, gamma, beta) gives.  B, C, groups <= 65535, eps > 0.
  * workspace: cutie_gn_workspace_bytes(B, HW, C, groups) bytes, 16-byte aligned, clobbered, no pre-fill.  B = 0 or HW = 0

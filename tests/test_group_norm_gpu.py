@@ -135,7 +135,7 @@ SHAPES = [
     (1, 1, 2, 3, 1, 1, 0),
     (2, 37, 53, 66, 6, 2, 0),        # eleven channels a group
     (2, 9, 7, 24, 2, 0, 0),          # twelve: 8-byte vectors of a 16-bit type, 16-byte of f32
-    (2, 9, 7, 64, 8, 0, 1),          # base off its 16-byte boundary: single elements
+    (2, 9, 7, 64, 8, 0, 1),          # base off its 16-byte boundary
     (2, 9, 7, 64, 8, 1, 0),          # odd leading dimension
     (1, 130, 130, 32, 2, 0, 0),      # a group too large for a workgroup
     (1, 130, 131, 33, 3, 0, 0),      # the same with single elements
@@ -169,6 +169,31 @@ def test_forward_and_backward(B, H, W, C, groups, pad, off, dtype):
         db3 = torch.full((C,), 7.0, device=DEV)
         ops.gn_bwd(dy, x, stats, dx3, gamma=gamma, beta=beta, act=act, dbeta=db3)
         assert torch.equal(db3, dbeta)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,W,C,groups,pad,off", [
+    (2, 128, 128, 16, 2, 0, 0),      # few groups of many pixels, which would fit: in slices all the same
+    (3, 64, 65, 66, 33, 1, 1),       # two channels a group
+    (24, 64, 64, 66, 33, 0, 0),      # and many of them
+    (1, 130, 130, 36, 2, 3, 1),      # slices of vectors that begin anywhere, groups that end inside a vector
+    (1, 61, 67, 1032, 4, 1, 0),      # wide rows: eight values a vector, more than one block of columns for f32
+    (2, 90, 91, 20, 1, 2, 1),
+])
+def test_forms_and_alignments(B, H, W, C, groups, pad, off, dtype):
+    x, dy, gamma, beta = make(B, H, W, C, groups, dtype, pad, off, seed=B + C)
+    y, stats = run_fwd(x, groups, gamma, beta, "silu")
+    check_fwd(x, groups, gamma, beta, "silu", y, stats)
+    wide = torch.full((B, H, W, C + pad + 1), 3.0, dtype=dtype, device=DEV)      # dx beside columns that stay
+    dgamma, dbeta = torch.full((C,), 7.0, device=DEV), torch.full((C,), 7.0, device=DEV)
+    ops.gn_bwd(dy, x, stats, wide[..., 1:C + 1], gamma=gamma, beta=beta, act="silu", dgamma=dgamma, dbeta=dbeta)
+    check_bwd(dy, x, stats, gamma, beta, "silu", wide[..., 1:C + 1], dgamma, dbeta)
+    assert bool((wide[..., 0] == 3).all()) and bool((wide[..., C + 1:] == 3).all())
+    again = torch.empty_like(dy)
+    dg2, db2 = torch.empty_like(dgamma), torch.empty_like(dbeta)
+    ops.gn_bwd(dy, x, stats, again, gamma=gamma, beta=beta, act="silu", dgamma=dg2, dbeta=db2)
+    assert torch.equal(again, wide[..., 1:C + 1]) and torch.equal(dg2, dgamma) and torch.equal(db2, dbeta)
 
 
 @pytest.mark.gpu
