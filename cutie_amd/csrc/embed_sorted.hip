@@ -4,8 +4,8 @@
 //   dtable[v][0:E] (+)= scale * sum of dout[cell][0:E] over the cells with ids[cell] == v, in the order of a stable sort
 //
 // Measured (MI355X), inputs that change from call to call: lookup 131072 x 128 f16 9 us, 500009 x 512 bf16 187 us (4.1 TB/s of the
-// 760 MB it must move; 156 us on the same inputs again); gradient 131072 x 128 f16, V 18000, 94 % of the cells on one id: 51 us in six
-// launches (27 us the two passes of the sort, 17 the sums, 9 the join); 500009 x 512 bf16, V 120000: 227 us, of which the sums 155
+// 760 MB it must move; 156 us on the same inputs again); gradient 131072 x 128 f16, V 18000, 94 % of the cells on one id: 49 us in six
+// launches (27 us the two passes of the sort, 15 the sums, 9 the join); 500009 x 512 bf16, V 120000: 227 us, of which the sums 155
 // (4.9 TB/s).
 //
 // The lookup is a row copy (HBM).  The gradient sorts (id, cell) pairs - a stable radix sort, least significant digit

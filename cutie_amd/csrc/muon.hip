@@ -17,7 +17,7 @@
 // a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
 // of a product is one 128-byte line of a row.  A and B [S][S] alike.
 //
-// Measured (MI355X), five steps: 14 filters (11 of them 3840 x 256) 428 us, of which the matrix cores need 110 for the three
+// Measured (MI355X), five steps: 14 filters (10 of them 3840 x 256) 411 - 428 us, of which the matrix cores need 110 for the three
 // products at the rate of a large library product; 2048 x 8192 1.84 ms (1.45 ms likewise; in f32 the library's rate gives 3.6).
 // There are three forms: the general one of this comment, and two for fewer columns, in f32, below.
 #include "conv_common.h"
