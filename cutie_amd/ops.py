@@ -75,8 +75,28 @@ def embed_bwd(ids, dout, dtable, workspace=None):
 
 # ------------------------------------------------------------------------------------ K16
 def _rows_ld(t):
-    """leading dimension of a [..., E] view whose leading axes collapse to one row index"""
-    return ld_of(t) if t.dim() > 1 and t.numel() else t.shape[-1]
+    """leading dimension of a [..., E] view whose leading axes collapse to one row index.  An axis of one element (and the
+    columns, where E is 1) says nothing by its stride: one row, one column or one sample of a larger tensor is a view like any"""
+    shape, strides = t.shape, t.stride()
+    E = shape[-1]
+    if not t.numel():
+        return E
+    if E > 1 and strides[-1] != 1:
+        raise capi.CutieError("channel axis must be contiguous")
+    ld = below = None      # below: elements that the axes behind the present one span
+    for d in range(len(shape) - 2, -1, -1):
+        if shape[d] == 1:
+            continue
+        if ld is None:
+            ld = strides[d]
+        elif strides[d] != below:
+            raise capi.CutieError("view is not row-collapsible: shape %s strides %s" % (tuple(shape), strides))
+        below = strides[d] * shape[d]
+    if ld is None:      # one row
+        return E
+    if ld > 0x7fffffff:      # an int in the C ABI
+        raise capi.CutieError("leading dimension %d is beyond 2^31 - 1" % ld)
+    return ld
 
 
 def _check_ids(what, ids, rows, table):
@@ -463,11 +483,6 @@ def _gn_views(what, x, stats, act, others):
     return B, HW, C
 
 
-def _gn_ld(t):
-    """ld_of, also for views with a dimension of one (their strides say nothing)"""
-    return ld_of(t) if t.shape[1] * t.shape[2] and t.shape[0] else t.shape[3]
-
-
 def gn_fwd(x, y, stats, gamma=None, beta=None, act=None, eps=GN_EPS, workspace=None):
     """Group norm with an activation (cutie_gn_fwd): y = act(gamma * (x - mean) * rstd + beta) over the C / groups channels and
     all pixels of a (sample, group).  x, y [B,H,W,C] views of one element type; stats f32 [B,groups,2] receives (mean, rstd) for
@@ -476,8 +491,8 @@ def gn_fwd(x, y, stats, gamma=None, beta=None, act=None, eps=GN_EPS, workspace=N
     B, HW, C = _gn_views("gn_fwd", x, stats, act, (y,))
     need = gn_workspace_bytes(B, HW, C, stats.shape[1])
     ws = _workspace(workspace, need, x.device, "gn_fwd")
-    call("cutie_gn_fwd", ptr(x), _gn_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_fwd: gamma")),
-         ptr(_f32_vec(beta, C, x.device, "gn_fwd: beta")), stats.shape[1], float(eps), GN_ACTIVATION_CODE[act], ptr(y), _gn_ld(y),
+    call("cutie_gn_fwd", ptr(x), _rows_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_fwd: gamma")),
+         ptr(_f32_vec(beta, C, x.device, "gn_fwd: beta")), stats.shape[1], float(eps), GN_ACTIVATION_CODE[act], ptr(y), _rows_ld(y),
          dt_of(x), ptr(stats), B, HW, C, ptr(ws), ws.numel() * ws.element_size(), stream())
     return y
 
@@ -488,8 +503,8 @@ def gn_bwd(dy, x, stats, dx, gamma=None, beta=None, act=None, dgamma=None, dbeta
     B, HW, C = _gn_views("gn_bwd", x, stats, act, (dy, dx))
     need = gn_workspace_bytes(B, HW, C, stats.shape[1])
     ws = _workspace(workspace, need, x.device, "gn_bwd")
-    call("cutie_gn_bwd", ptr(dy), _gn_ld(dy), ptr(x), _gn_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_bwd: gamma")),
-         ptr(_f32_vec(beta, C, x.device, "gn_bwd: beta")), stats.shape[1], GN_ACTIVATION_CODE[act], ptr(stats), ptr(dx), _gn_ld(dx),
+    call("cutie_gn_bwd", ptr(dy), _rows_ld(dy), ptr(x), _rows_ld(x), ptr(_f32_vec(gamma, C, x.device, "gn_bwd: gamma")),
+         ptr(_f32_vec(beta, C, x.device, "gn_bwd: beta")), stats.shape[1], GN_ACTIVATION_CODE[act], ptr(stats), ptr(dx), _rows_ld(dx),
          dt_of(x), ptr(_f32_vec(dgamma, C, x.device, "gn_bwd: dgamma")), ptr(_f32_vec(dbeta, C, x.device, "gn_bwd: dbeta")),
          1 if accumulate else 0, B, HW, C, ptr(ws), ws.numel() * ws.element_size(), stream())
     return dx
