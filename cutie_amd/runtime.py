@@ -339,6 +339,8 @@ class Engine(object):
         P.wgrad_ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         P.scratch = torch.zeros(capi.REDUCE_SCRATCH, dtype=torch.float32, device=dev)
         P.hnm_ws = torch.empty(ops.hnm_workspace_bytes(B * P.H * P.W), dtype=torch.uint8, device=dev)
+        P.embed_ws = {}      # one per embedding: its size is the table's and the form's
+        P.emb_part = torch.zeros(1, dtype=torch.float32, device=dev)
         P.reg = torch.zeros(1, dtype=torch.float32, device=dev)
         P.gnorm_sq = torch.zeros(1, dtype=torch.float32, device=dev)
         P.bwd_ready = True
@@ -685,6 +687,7 @@ class Engine(object):
         defer = self.wgrad_batch and side is None
         pending = []
         pending_elems = [0]
+        P.embed_rows = []      # (gradient of the looked-up rows, factor of the rows) of every embedding
 
         def flush():
             if not pending:
@@ -753,17 +756,17 @@ class Engine(object):
             elif n.op == "embed":
                 self._backprop_into(P, n)
                 by_sort = self.embed_sorted or _scale(n) != 1.0
-                if getattr(P, "embed_ws", None) is None:
+                if n.name not in P.embed_ws:
                     need = (ops.embed_grad_sorted_workspace_bytes(P.grid.numel(), n.attrs["V"], n.channels) if by_sort else
                             ops.embed_bwd_workspace_bytes(P.grid.numel(), n.channels))
-                    P.embed_ws = torch.empty(need, dtype=torch.uint8, device=self.dev)
-                dw = self.grads[n.name + "/weights"]
+                    P.embed_ws[n.name] = torch.empty(need, dtype=torch.uint8, device=self.dev)
+                dw, ws = self.grads[n.name + "/weights"], P.embed_ws[n.name]
                 if by_sort:
-                    ops.embed_grad_sorted(P.grid, P.dy[n.name][..., :n.channels], dw, scale=_scale(n), workspace=P.embed_ws)
+                    ops.embed_grad_sorted(P.grid, P.dy[n.name][..., :n.channels], dw, scale=_scale(n), workspace=ws)
                 else:
-                    ops.embed_bwd(P.grid, P.dy[n.name][..., :n.channels], dw, P.embed_ws)
+                    ops.embed_bwd(P.grid, P.dy[n.name][..., :n.channels], dw, ws)
                 P.d_embed = P.dy[n.name]
-                P.embed_scale = _scale(n)
+                P.embed_rows.append((P.d_embed, _scale(n)))
         flush()
         if side is not None:
             main.wait_stream(side)     # every weight gradient is in place; the buffers it read may be reused
@@ -814,11 +817,10 @@ class Engine(object):
             self._muon_names = [k for k in names if k not in adam]
             self._muon_plan = None
         rows = None
-        if emb_rows_sq is None and hasattr(P, "d_embed"):
-            if P.embed_scale == 1.0:
-                rows = P.d_embed.reshape(-1)
-            else:
-                emb_rows_sq = self.embedding_rows_sumsq(P)      # rows of the table's gradient: scale times d_embed
+        if emb_rows_sq is None and P.embed_rows:
+            rows = self._plain_rows(P)
+            if rows is None:
+                emb_rows_sq = self.embedding_rows_sumsq(P)
         ops.opt_norm(self.params_flat, self.grads_flat, self.n_conv_w, self.n_dense, wd * world, self._opt_partials,
                      rows=rows, loss_scale=self.loss_scale)
         ops.opt_step(self.params_flat, self.grads_flat, m, v, self.n_conv_w, wd * world, 0.5 * wd, self._opt_layers, self.dt,
@@ -881,11 +883,19 @@ class Engine(object):
         share of tf.clip_by_global_norm (IndexedSlices values, un-deduplicated).  A 1-float device tensor."""
         P.emb_sq = self.grads_extra      # rides behind the gradient buffer (GradBuckets.finish(tail_extra=1))
         P.emb_sq.zero_()
-        if hasattr(P, "d_embed"):
-            ops.sumsq(P.d_embed.reshape(-1), P.emb_sq, P.scratch, self.loss_scale)     # still scaled: activation dtype
-            if P.embed_scale != 1.0:
-                P.emb_sq.mul_(P.embed_scale ** 2)
+        for k, (rows, scale) in enumerate(P.embed_rows):
+            sq = P.emb_part.zero_() if k else P.emb_sq
+            ops.sumsq(rows.reshape(-1), sq, P.scratch, self.loss_scale)     # still scaled: activation dtype
+            if scale != 1.0:
+                sq.mul_(scale ** 2)      # rows of the table's gradient: scale times the looked-up rows' gradient
+            if k:
+                P.emb_sq.add_(sq)
         return P.emb_sq
+
+    @staticmethod
+    def _plain_rows(P):
+        """the looked-up rows' gradient where it is the whole of embedding_rows_sumsq's: one embedding, no factor"""
+        return P.embed_rows[0][0].reshape(-1) if len(P.embed_rows) == 1 and P.embed_rows[0][1] == 1.0 else None
 
     def global_norm_sq(self, P, tf_indexed_slices=True, embedding_rows_sq=None):
         """Squared global norm the way tf.clip_by_global_norm sees it: every dense gradient, and the
@@ -896,13 +906,14 @@ class Engine(object):
         if embedding_rows_sq is not None:
             ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
             P.gnorm_sq.add_(embedding_rows_sq)
-        elif tf_indexed_slices and hasattr(P, "d_embed") and P.embed_scale != 1.0:
-            rows = self.embedding_rows_sumsq(P)
+        elif tf_indexed_slices and P.embed_rows:
+            rows = self._plain_rows(P)
+            sq = self.embedding_rows_sumsq(P) if rows is None else None
             ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
-            P.gnorm_sq.add_(rows)
-        elif tf_indexed_slices and hasattr(P, "d_embed"):
-            ops.sumsq(self.grads_flat[:self.n_dense], P.gnorm_sq, P.scratch)
-            ops.sumsq(P.d_embed.reshape(-1), P.gnorm_sq, P.scratch, self.loss_scale)   # still scaled: activation dtype
+            if rows is None:
+                P.gnorm_sq.add_(sq)
+            else:
+                ops.sumsq(rows, P.gnorm_sq, P.scratch, self.loss_scale)   # still scaled: activation dtype
         else:
             ops.sumsq(self.grads_flat, P.gnorm_sq, P.scratch)
         return P.gnorm_sq
