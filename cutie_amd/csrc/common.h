@@ -57,6 +57,22 @@ int device_cus();      // compute units of the current device, 0 when unknown
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Arguments of one call that may not share a byte.  Dense: `bytes` at p (NULL meets nothing).
+struct Dense { const void* p; uint64_t bytes; };
+static inline bool dense_meet(Dense a, Dense b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+// Rows: `rows` of `width` bytes, one every `step`; what lies between them is not theirs.
+struct Rows { const void* p; int64_t rows; uint64_t width, step; };
+static inline bool rows_meet(Rows r, Dense d) {
+    if (r.rows < 1 || !dense_meet(Dense{r.p, (uint64_t)(r.rows - 1) * r.step + r.width}, d)) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(r.p), y = reinterpret_cast<uintptr_t>(d.p);
+    if (y <= x) return true;      // over the first row's first byte
+    const uint64_t at = (y - x) % r.step;
+    return at < r.width || at + d.bytes > r.step;      // in a row, or into the next one
+}
+
 typedef unsigned short bf16_t;  // raw bits
 
 // round-to-nearest-even f32 -> bf16 (NaN stays NaN): lowers to v_cvt_pk_bf16_f32 on gfx950

@@ -763,6 +763,18 @@ inline bool gn_overlap(const void* a, int ld_a, const void* b, int ld_b, int64_t
     return d < (uintptr_t)C * es || row - d < (uintptr_t)C * es;
 }
 
+// the outputs beside the activations (`outs`; the workspace, where the form uses one) meet no other tensor of the call
+inline int gn_apart(const char* who, const Rows* views, int nv, const Dense* ins, int ni, const Dense* outs, int no) {
+    bool bad = false;
+    for (int i = 0; i < no; ++i) {
+        for (int j = 0; j < nv; ++j) bad |= rows_meet(views[j], outs[i]);
+        for (int j = 0; j < ni; ++j) bad |= dense_meet(ins[j], outs[i]);
+        for (int j = 0; j < i; ++j) bad |= dense_meet(outs[j], outs[i]);
+    }
+    CUTIE_CHECK_ARG(!bad, "%s: statistics, gradients of gamma and beta or the workspace overlaps another tensor of the call", who);
+    return CUTIE_OK;
+}
+
 inline int gn_check(const char* who, int B, int HW, int C, int G, int act, int dt) {
     CUTIE_CHECK_ARG(B >= 0 && HW >= 0 && C >= 1 && G >= 1 && C % G == 0, "%s: B=%d HW=%d C=%d groups=%d (groups must divide C)", who, B,
                     HW, C, G);
@@ -793,9 +805,20 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
                     "gn_fwd: misaligned pointers");
     const int vec = gn_vec(dtype, C / groups);
     const GnPlan p = gn_plan(B, HW, C, groups, dtype, vec, GN_FWD_KMAX, 1024, false);
-    const bool lap = gn_overlap(x, ld_x, y, ld_y, (int64_t)B * HW, C, elem_bytes(dtype));
+    const GnSpace w = gn_space(B, HW, C, groups);
+    if (!p.resident && (!workspace || workspace_bytes < w.total || !aligned16(workspace))) {
+        set_error("gn_fwd: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
+        return CUTIE_E_WORKSPACE;
+    }
+    const int es = elem_bytes(dtype);
+    CUTIE_CHECK_ARG(!gn_overlap(x, ld_x, y, ld_y, (int64_t)B * HW, C, es), "gn_fwd: y overlaps x");
+    const uint64_t vector = (uint64_t)C * sizeof(float), width = (uint64_t)C * es;
+    const Rows views[] = {{x, (int64_t)B * HW, width, (uint64_t)ld_x * es}, {y, (int64_t)B * HW, width, (uint64_t)ld_y * es}};
+    const Dense ins[] = {{gamma, vector}, {beta, vector}};
+    const Dense outs[] = {{stats, (uint64_t)B * groups * 2 * sizeof(float)}, {p.resident ? nullptr : workspace, w.total}};
+    if (int e = gn_apart("gn_fwd", views, 2, ins, 2, outs, 2)) return e;
+    CUTIE_CHECK_ARG(!rows_meet(views[1], ins[0]) && !rows_meet(views[1], ins[1]), "gn_fwd: y overlaps gamma or beta");
     if (p.resident) {
-        CUTIE_CHECK_ARG(!lap, "gn_fwd: y overlaps x");
         const dim3 grid((unsigned)(cdiv(p.s.items, 8) * 8));
         CUTIE_DISPATCH_DTYPE(dtype, DT, {
             typedef typename elem<DT>::type E;
@@ -812,12 +835,6 @@ extern "C" int cutie_gn_fwd(const void* x, int ld_x, const float* gamma, const f
         CUTIE_CHECK_LAUNCH();
         return CUTIE_OK;
     }
-    const GnSpace w = gn_space(B, HW, C, groups);
-    if (!workspace || workspace_bytes < w.total || !aligned16(workspace)) {
-        set_error("gn_fwd: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
-        return CUTIE_E_WORKSPACE;
-    }
-    CUTIE_CHECK_ARG(!lap, "gn_fwd: y overlaps x");
     char* ws = (char*)workspace;
     double* slots = (double*)(ws + w.slots);
     float* low = (float*)(ws + w.low);
@@ -857,6 +874,14 @@ extern "C" int cutie_gn_bwd(const void* dy, int ld_dy, const void* x, int ld_x, 
     }
     CUTIE_CHECK_ARG(none || !(gn_overlap(dy, ld_dy, dx, ld_dx, (int64_t)B * HW, C, es) || gn_overlap(x, ld_x, dx, ld_dx, (int64_t)B * HW, C, es)),
                     "gn_bwd: dx overlaps dy or x");
+    const uint64_t vector = (uint64_t)C * sizeof(float), width = (uint64_t)C * es;
+    const int64_t rows = (int64_t)B * HW;      // 0: no views
+    const Rows views[] = {{dy, rows, width, (uint64_t)ld_dy * es}, {x, rows, width, (uint64_t)ld_x * es}, {dx, rows, width, (uint64_t)ld_dx * es}};
+    const Dense ins[] = {{gamma, vector}, {beta, vector}, {stats, (uint64_t)B * groups * 2 * sizeof(float)}};
+    const Dense outs[] = {{dgamma, vector}, {dbeta, vector}, {none ? nullptr : workspace, w.total}};
+    if (int e = gn_apart("gn_bwd", views, 3, ins, 3, outs, 3)) return e;
+    CUTIE_CHECK_ARG(!rows_meet(views[2], ins[0]) && !rows_meet(views[2], ins[1]) && !rows_meet(views[2], ins[2]),
+                    "gn_bwd: dx overlaps gamma, beta or stats");
     char* ws = (char*)workspace;
     float* chan = ws ? (float*)(ws + w.chan) : nullptr;
     if (!none) {

@@ -1,0 +1,93 @@
+"""Calls of the training operators in which an output shares memory with another tensor are refused on the host, before anything is
+launched: made-up addresses, no GPU.  (Tensors that only lie in the gaps between the rows of a view are neighbours, not overlaps.)
+"""
+import ctypes
+
+import pytest
+import torch
+
+from cutie_amd import capi, ops
+
+A = ctypes.c_void_p
+FAR = [1 << k for k in range(36, 46)]      # addresses that meet nothing
+
+
+def refused(rc):
+    return rc == -1 and b"overlaps" in capi.lib().cutie_last_error()
+
+
+# ------------------------------------------------------------------------------------------------------------------ group norm
+# B 2, HW 4, C 8 f32, 2 groups: rows of 32 bytes, 64 apart (ld 16): a view covers 64 * 7 + 32 = 480 bytes; stats 32, vectors 32
+def gn_fwd(HW=4, **kw):
+    a = dict(x=FAR[0], gamma=FAR[1], beta=FAR[2], y=FAR[3], stats=FAR[4], ws=FAR[5])
+    a.update(kw)
+    return capi.lib().cutie_gn_fwd(A(a["x"]), 16, A(a["gamma"]), A(a["beta"]), 2, 1e-5, 0, A(a["y"]), 16, 0, A(a["stats"]), 2, HW, 8,
+                                   A(a["ws"]), 1 << 30, None)
+
+
+def gn_bwd(**kw):
+    a = dict(dy=FAR[0], x=FAR[1], gamma=FAR[2], beta=FAR[3], stats=FAR[4], dx=FAR[5], dgamma=FAR[6], dbeta=FAR[7], ws=FAR[8], B=2)
+    a.update(kw)
+    return capi.lib().cutie_gn_bwd(A(a["dy"]), 16, A(a["x"]), 16, A(a["gamma"]), A(a["beta"]), 2, 0, A(a["stats"]), A(a["dx"]), 16, 0,
+                                   A(a["dgamma"]), A(a["dbeta"]), 0, a["B"], 4, 8, A(a["ws"]), 1 << 20, None)
+
+
+VIEW_OFFSETS = (-28, 0, 28, 64, 448 + 28, 32 + 4)      # the last one begins in a gap and runs into the next row
+
+
+@pytest.mark.parametrize("off", VIEW_OFFSETS)
+@pytest.mark.parametrize("view", ["x", "y"])
+def test_group_norm_forward_statistics_over_a_view(view, off):
+    assert refused(gn_fwd(stats=FAR[0 if view == "x" else 3] + off))
+
+
+@pytest.mark.parametrize("kw", [dict(stats=FAR[1] + 28), dict(stats=FAR[2] - 28), dict(gamma=FAR[3] + 64), dict(beta=FAR[3] - 4)])
+def test_group_norm_forward_vectors(kw):
+    assert refused(gn_fwd(**kw))
+
+
+@pytest.mark.parametrize("over", ["x", "y", "gamma", "beta", "stats"])
+def test_group_norm_forward_workspace(over):
+    """the form that goes through the workspace"""
+    assert refused(gn_fwd(HW=1 << 20, **{over: FAR[5] + 64}))
+
+
+@pytest.mark.parametrize("off", VIEW_OFFSETS)
+@pytest.mark.parametrize("view", ["dy", "x", "dx"])
+@pytest.mark.parametrize("out", ["dgamma", "dbeta"])
+def test_group_norm_backward_vectors_over_a_view(out, view, off):
+    at = dict(dy=FAR[0], x=FAR[1], dx=FAR[5])
+    assert refused(gn_bwd(**{out: at[view] + off}))
+
+
+@pytest.mark.parametrize("out", ["dgamma", "dbeta"])
+@pytest.mark.parametrize("other", ["gamma", "beta", "stats"])
+def test_group_norm_backward_vectors(out, other):
+    at = dict(gamma=FAR[2], beta=FAR[3], stats=FAR[4])
+    assert refused(gn_bwd(**{out: at[other] + 28})) and refused(gn_bwd(**{out: at[other]}))
+    assert refused(gn_bwd(**{other: FAR[5] + 64}))      # dx over it
+
+
+def test_group_norm_backward_one_gradient_twice():
+    assert refused(gn_bwd(dgamma=FAR[7])) and refused(gn_bwd(dbeta=FAR[6] + 28)) and refused(gn_bwd(dgamma=FAR[7], B=0))
+
+
+@pytest.mark.parametrize("over", ["dy", "x", "gamma", "beta", "stats", "dx", "dgamma", "dbeta"])
+def test_group_norm_backward_workspace(over):
+    assert refused(gn_bwd(**{over: FAR[8] + 64}))
+
+
+@pytest.mark.gpu
+def test_group_norm_neighbours_are_taken():
+    """statistics and gradients in the gaps between the rows of the views"""
+    wide = torch.randn(2, 4, 1, 16, generator=torch.Generator().manual_seed(1)).to("cuda:0")
+    x, dy = wide[..., :8].clone(), wide[..., 8:].clone()
+    y, st, dx, dg, db = torch.empty_like(x), torch.empty(2, 2, 2, device="cuda:0"), torch.empty_like(x), torch.empty(8, device="cuda:0"), torch.empty(8, device="cuda:0")
+    ops.gn_fwd(x, y, st)
+    ops.gn_bwd(dy, x, st, dx, dgamma=dg, dbeta=db)
+    s2 = wide.view(-1)[8:16].view(2, 2, 2)      # the gap behind the first row
+    ops.gn_fwd(wide[..., :8], dx.clone(), s2)
+    assert torch.equal(s2, st)
+    g2, b2, out = wide.view(-1)[24:32], wide.view(-1)[40:48], torch.empty_like(dx)
+    ops.gn_bwd(dy, wide[..., :8], st, out, dgamma=g2, dbeta=b2)
+    assert torch.equal(out, dx) and torch.equal(g2, dg) and torch.equal(b2, db)
