@@ -635,6 +635,10 @@ extern "C" int cutie_embed_scaled_fwd(const int32_t* ids, int64_t n_cells, const
     const int es = out_dtype == CUTIE_F32 ? 4 : 2;
     CUTIE_CHECK_ARG(((uintptr_t)out % es) == 0 && ((uintptr_t)table % 4) == 0 && ((uintptr_t)ids % 4) == 0,
                     "embed_scaled_fwd: misaligned pointers");
+    const Dense in_ids{ids, (uint64_t)n_cells * 4}, in_table{table, (uint64_t)V * E * 4}, count{oob_count, 4};
+    const Rows rows_out{out, n_cells, (uint64_t)E * es, (uint64_t)ld_out * es};
+    CUTIE_CHECK_ARG(!rows_meet(rows_out, in_ids) && !rows_meet(rows_out, in_table) && !rows_meet(rows_out, count) &&
+                        !dense_meet(count, in_ids) && !dense_meet(count, in_table), "embed_scaled_fwd: an output overlaps another tensor of the call");
     const int vec = row_vec(out_dtype, E, table);
     const int cv = E / vec, rows = 256 / (cv < 256 ? cv : 256);
     int64_t g = cdiv(n_cells, (int64_t)rows * 4);
@@ -674,6 +678,10 @@ extern "C" int cutie_embed_grad_sorted(const int32_t* ids, int64_t n_cells, cons
         set_error("embed_grad_sorted: workspace %zu < %zu (or not 16-byte aligned)", workspace ? workspace_bytes : 0, w.total);
         return CUTIE_E_WORKSPACE;
     }
+    const Dense in_ids{ids, (uint64_t)n_cells * 4}, space{workspace, w.total}, sums{dtable, (uint64_t)V * E * 4};
+    const Rows rows_in{dout, n_cells, (uint64_t)E * es, (uint64_t)ld_dout * es};
+    CUTIE_CHECK_ARG(!rows_meet(rows_in, sums) && !rows_meet(rows_in, space) && !dense_meet(in_ids, sums) && !dense_meet(in_ids, space) &&
+                        !dense_meet(sums, space), "embed_grad_sorted: dtable or the workspace overlaps another tensor of the call");
     if (n_cells == 0 && accumulate) return CUTIE_OK;
     char* ws = (char*)workspace;
     const SortPlan sp = sort_plan(n_cells, V);

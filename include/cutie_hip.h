@@ -112,6 +112,7 @@ int cutie_embed_bwd(const int32_t* ids, int64_t n_cells, const void* dout, int l
  *       (zeros where no cell has the id), else the sums are added to what is there and other rows are left alone.  An id
  *       outside [0, V) adds to nothing.  The cells are ordered by a stable sort on the id and every row has one owner: f32
  *       sums in an order that ids, V, E, the type and the table's alignment fix, no atomics, the same bits every run.
+ * An output or the workspace may not overlap another tensor of the call (dtable among the gaps between dout's rows is fine).
  * E = 1 .. 65536, n_cells <= 2^30, V < 2^30; views whose base and leading dimension are multiples of 16 bytes move fastest.
  * workspace: cutie_embed_grad_sorted_workspace_bytes(n_cells, V, E) bytes, 16-byte aligned, clobbered, no pre-fill. */
 int cutie_embed_scaled_fwd(const int32_t* ids, int64_t n_cells, const float* table, int V, int E, float scale,

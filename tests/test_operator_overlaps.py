@@ -91,3 +91,43 @@ def test_group_norm_neighbours_are_taken():
     g2, b2, out = wide.view(-1)[24:32], wide.view(-1)[40:48], torch.empty_like(dx)
     ops.gn_bwd(dy, wide[..., :8], st, out, dgamma=g2, dbeta=b2)
     assert torch.equal(out, dx) and torch.equal(g2, dg) and torch.equal(b2, db)
+
+
+# ------------------------------------------------------------------------------------------------------------------ embedding
+# 4 cells, rows of 8 f32 (32 bytes) 64 apart; a table of 3 x 8 (96 bytes), ids 16 bytes
+def lookup(**kw):
+    a = dict(ids=FAR[0], table=FAR[1], out=FAR[2], oob=FAR[3])
+    a.update(kw)
+    return capi.lib().cutie_embed_scaled_fwd(A(a["ids"]), 4, A(a["table"]), 3, 8, 1.0, A(a["out"]), 16, 0, A(a["oob"]), None)
+
+
+def gradient(n=4, **kw):
+    a = dict(ids=FAR[0], dout=FAR[1], dtable=FAR[2], ws=FAR[3])
+    a.update(kw)
+    return capi.lib().cutie_embed_grad_sorted(A(a["ids"]), n, A(a["dout"]), 16, 0, 1.0, A(a["dtable"]), 3, 8, 0, A(a["ws"]), 1 << 20, None)
+
+
+@pytest.mark.parametrize("kw", [dict(ids=FAR[2] + 64), dict(ids=FAR[2] - 12), dict(table=FAR[2]), dict(table=FAR[2] - 92), dict(table=FAR[2] + 32),
+                                dict(oob=FAR[2] + 28), dict(oob=FAR[0] + 12), dict(oob=FAR[1] + 92)])
+def test_lookup(kw):
+    assert refused(lookup(**kw))
+
+
+@pytest.mark.parametrize("kw", [dict(dtable=FAR[0] + 12), dict(dtable=FAR[0] - 92), dict(dtable=FAR[1]), dict(dtable=FAR[1] + 32), dict(dtable=FAR[1] + 192 + 28),
+                                dict(ids=FAR[3] + 16), dict(dout=FAR[3] + 16), dict(dtable=FAR[3] + 16), dict(dout=FAR[3] - 64)])
+def test_gradient(kw):
+    assert refused(gradient(**kw))
+
+
+@pytest.mark.gpu
+def test_embedding_neighbours_are_taken():
+    """the gradient's table as columns beside the rows it is made from: a table of one row in one gap"""
+    wide = torch.randn(4, 16, generator=torch.Generator().manual_seed(2)).to("cuda:0")
+    ids = torch.tensor([0, 1, 0, -1], dtype=torch.int32, device="cuda:0")
+    want = wide[0, :8] + wide[2, :8]
+    got = wide[1:2, 8:]
+    assert ops.embed_grad_sorted(ids, wide[:, :8], got) is got and torch.equal(got[0], want)
+    oob = wide[3, 8:9].view(torch.int32)
+    oob.zero_()
+    ops.embed_scaled_fwd(ids, got, wide[:, :8], 2.0, oob)
+    assert torch.equal(wide[0, :8], 2 * want) and torch.equal(wide[2, :8], 2 * want) and int(oob) == 2 and not wide[1, :8].any()
