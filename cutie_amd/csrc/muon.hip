@@ -1087,20 +1087,19 @@ inline int ns_common(const char* who, int steps, float eps, const NsPlan& p, con
 inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // An output may be the input of its own place (ins[in]), and shares no byte with any other tensor of the call.
-struct Span { const float* p; int64_t n; };
-struct Target { const float* p; int in; int64_t n; };
-inline bool meet(const float* a, int64_t na, const float* b, int64_t nb) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + (uintptr_t)nb * 4 && y < x + (uintptr_t)na * 4;
-}
-inline int ns_disjoint(const char* who, const Target* outs, int no, const Span* ins, int ni, int per) {
+struct Target { Dense t; int in; };
+inline int ns_disjoint(const char* who, const Target* outs, int no, const Dense* ins, int ni, int per, Dense space) {
     for (int i = 0; i < no; ++i) {
         const Target& o = outs[i];
         bool bad = false;
-        for (int j = 0; j < i; ++j) bad |= meet(o.p, o.n, outs[j].p, outs[j].n);
-        for (int j = 0; j < ni; ++j) bad |= meet(o.p, o.n, ins[j].p, ins[j].n) && !(j == o.in && ins[j].p == o.p);
+        for (int j = 0; j < i; ++j) bad |= dense_meet(o.t, outs[j].t);
+        for (int j = 0; j < ni; ++j) bad |= dense_meet(o.t, ins[j]) && !(j == o.in && ins[j].p == o.t.p);
         CUTIE_CHECK_ARG(!bad, "%s: matrix %d: an output overlaps another tensor of the call", who, i / per);
     }
+    bool bad = false;
+    for (int i = 0; i < no; ++i) bad |= dense_meet(space, outs[i].t);
+    for (int j = 0; j < ni; ++j) bad |= dense_meet(space, ins[j]);
+    CUTIE_CHECK_ARG(!bad, "%s: the workspace overlaps another tensor of the call", who);
     return CUTIE_OK;
 }
 }  // namespace
@@ -1127,14 +1126,14 @@ extern "C" int cutie_orthogonalize_batched(const cutie_orth_desc* descs, int n, 
     NsPlan p;
     if (int e = ns_plan("orthogonalize", shapes, n, p)) return e;
     if (int e = ns_common("orthogonalize", steps, eps, p, workspace, workspace_bytes)) return e;
-    Span ins[CUTIE_MAX_BATCH];
+    Dense ins[CUTIE_MAX_BATCH];
     Target outs[CUTIE_MAX_BATCH];
     for (int i = 0; i < n; ++i) {
-        const int64_t size = (int64_t)descs[i].rows * descs[i].cols;
-        ins[i] = Span{descs[i].g, size};
-        outs[i] = Target{descs[i].out, i, size};
+        const uint64_t size = (uint64_t)descs[i].rows * descs[i].cols * sizeof(float);
+        ins[i] = Dense{descs[i].g, size};
+        outs[i] = Target{{descs[i].out, size}, i};
     }
-    if (int e = ns_disjoint("orthogonalize", outs, n, ins, n, 1)) return e;
+    if (int e = ns_disjoint("orthogonalize", outs, n, ins, n, 1, Dense{workspace, p.bytes})) return e;
     Hyper h = {};
     return ns_run<false>(p, ios, h, steps, eps, (char*)workspace, (hipStream_t)stream_);
 }
@@ -1157,18 +1156,21 @@ extern "C" int cutie_muon_step(const cutie_muon_desc* descs, int n, float lr, fl
     NsPlan p;
     if (int e = ns_plan("muon_step", shapes, n, p)) return e;
     if (int e = ns_common("muon_step", steps, eps, p, workspace, workspace_bytes)) return e;
-    Span ins[3 * CUTIE_MAX_BATCH];
+    Dense ins[3 * CUTIE_MAX_BATCH + 3];
     Target outs[2 * CUTIE_MAX_BATCH];
     for (int i = 0; i < n; ++i) {
         const cutie_muon_desc& d = descs[i];
-        const int64_t size = (int64_t)d.rows * d.cols;
-        ins[3 * i] = Span{d.p, size};
-        ins[3 * i + 1] = Span{d.g, size};
-        ins[3 * i + 2] = Span{d.m, size};
-        outs[2 * i] = Target{d.p_out, 3 * i, size};
-        outs[2 * i + 1] = Target{d.m_out, 3 * i + 2, size};
+        const uint64_t size = (uint64_t)d.rows * d.cols * sizeof(float);
+        ins[3 * i] = Dense{d.p, size};
+        ins[3 * i + 1] = Dense{d.g, size};
+        ins[3 * i + 2] = Dense{d.m, size};
+        outs[2 * i] = Target{{d.p_out, size}, 3 * i};
+        outs[2 * i + 1] = Target{{d.m_out, size}, 3 * i + 2};
     }
-    if (int e = ns_disjoint("muon_step", outs, 2 * n, ins, 3 * n, 2)) return e;
+    ins[3 * n] = Dense{gnorm_sq, 4};
+    ins[3 * n + 1] = Dense{loss_scale, 8};
+    ins[3 * n + 2] = Dense{invalid, 4};
+    if (int e = ns_disjoint("muon_step", outs, 2 * n, ins, 3 * n + 3, 2, Dense{workspace, p.bytes})) return e;
     const Hyper h = {lr, momentum, weight_decay, l2, clip, grad_scale, nesterov, gnorm_sq, loss_scale, invalid};
     return ns_run<true>(p, ios, h, steps, eps, (char*)workspace, (hipStream_t)stream_);
 }

@@ -548,9 +548,9 @@ int cutie_opt_step(float* p, float* g, float* m, float* v, int64_t n, int64_t n_
  * muon_step:  g' = (g / S + l2 * p) * grad_scale * (clip > 0 ? clip / max(sqrt(*gnorm_sq) * grad_scale, clip) : 1)
  *     m_out = momentum * m + g';   u = nesterov ? g' + momentum * m_out : m_out
  *     p_out = p * (1 - lr * weight_decay) - lr * out_scale * orthogonalize(u)
- *     p_out may be its own p, m_out its own m; an output overlaps nothing else of the call.  S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq
- *     (nullable; the squared norm with S taken out, as cutie_opt_step leaves it) that is not finite or *invalid != 0 (nullable)
- *     makes p_out = p, m_out = m.
+ *     p_out may be its own p, m_out its own m; an output overlaps nothing else of the call, the workspace nothing at all.
+ *     S = loss_scale[0] of K12's state (nullable: 1).  A *gnorm_sq (nullable; the squared norm with S taken out, as cutie_opt_step
+ *     leaves it) that is not finite or *invalid != 0 (nullable) makes p_out = p, m_out = m.
  * The products run on the matrix cores at f32 accuracy: operands are two f16 (22 bits), sums f32, sums of squares f64, all in a
  * fixed order: the same bits every run for one list of shapes (a matrix's bits depend on the others of its call: K is cut by
  * their number).  X is kept to 2^-36 there: of a matrix whose norm lies far below eps, less of the (then small) result is left.

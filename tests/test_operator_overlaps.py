@@ -131,3 +131,34 @@ def test_embedding_neighbours_are_taken():
     oob.zero_()
     ops.embed_scaled_fwd(ids, got, wide[:, :8], 2.0, oob)
     assert torch.equal(wide[0, :8], 2 * want) and torch.equal(wide[2, :8], 2 * want) and int(oob) == 2 and not wide[1, :8].any()
+
+
+# ------------------------------------------------------------------------------------------------------------------ the update
+def muon(scalars, ws=1 << 20, at=4096):
+    d = capi.MuonDesc()
+    d.p, d.g, d.m, d.p_out, d.m_out = (at + 1024 * k for k in range(5))
+    d.rows, d.cols, d.out_scale = 16, 16, 1.0      # 1024 bytes each
+    a = dict(gnorm_sq=FAR[0], loss_scale=FAR[1], invalid=FAR[2])
+    a.update(scalars)
+    return capi.lib().cutie_muon_step(ctypes.byref(d), 1, 0.1, 0.9, 1, 0.0, 0.0, 5, 1e-7, A(a["gnorm_sq"]), 1.0, 1.0, A(a["loss_scale"]),
+                                      A(a["invalid"]), A(ws), 1 << 40, None)
+
+
+@pytest.mark.parametrize("name", ["gnorm_sq", "loss_scale", "invalid"])
+@pytest.mark.parametrize("off", [3 * 1024, 3 * 1024 + 1020, 4 * 1024, 5 * 1024 - 4])
+def test_update_over_what_it_is_steered_by(name, off):
+    assert refused(muon({name: 4096 + off}))
+
+
+def test_update_workspace():
+    for k in range(5):
+        assert refused(muon({}, at=(1 << 20) - 1024 * k + 128 if k else (1 << 20) + 128))
+    for name, size in (("gnorm_sq", 4), ("loss_scale", 8), ("invalid", 4)):
+        assert refused(muon({name: (1 << 20) + 4})) and refused(muon({name: (1 << 20) + 4 - size}))
+
+
+@pytest.mark.parametrize("g,out", [((1 << 20) + 128, FAR[0]), (FAR[0], (1 << 20) + 128), (FAR[0], (1 << 20) - 64)])
+def test_orthogonalize_workspace(g, out):
+    d = capi.OrthDesc()
+    d.g, d.out, d.rows, d.cols = g, out, 16, 16
+    assert refused(capi.lib().cutie_orthogonalize_batched(ctypes.byref(d), 1, 5, 1e-7, A(1 << 20), 1 << 40, None))
