@@ -723,7 +723,9 @@ inline GnPlan gn_plan(int B, int HW, int C, int G, int dt, int vec, int kmax, in
     p.K = (int)cdiv(HW, p.s.rows_par);
     auto pow2 = [](int64_t v) { return v <= 64 && (v & (v - 1)) == 0; };
     p.s.fast = pow2(cv) && pow2(cv / gc);
-    p.resident = p.K <= kmax && p.s.items <= (1 << 30) && gn_resident_us(p.s, es, bwd) <= gn_split_us((int64_t)B * HW * C * es, bwd);
+    // a launch counts its threads in 32 bits (20000 x 1 x 45023 f16 in 4093 groups: 82 million workgroups of 64)
+    const bool launches = cdiv(p.s.items, 8) * 8 * p.threads <= 0xffffffffll;
+    p.resident = p.K <= kmax && launches && gn_resident_us(p.s, es, bwd) <= gn_split_us((int64_t)B * HW * C * es, bwd);
     return p;
 }
 
