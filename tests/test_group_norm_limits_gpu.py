@@ -34,3 +34,57 @@ def test_more_groups_than_a_launch_has_threads():
     ref, _, _, mag, _, _ = gn.gn_bwd64(dy[at].cpu(), xs.cpu(), ss.cpu(), None, None, "none")
     tol = 2.0 ** -11 * ref.abs() * (1 + 2.0 ** -11) + (512 * U + 2.0 ** -20) * mag + 2.0 ** -25
     assert bool(((dx[at].cpu().double() - ref).abs() <= tol).all())
+
+
+# a plane in slices (16 channels a group, 270400 values), eleven channels a group, one with 16-byte vectors that span groups
+SLICED = [(1, 130, 130, 32, 2), (1, 130, 131, 33, 3), (2, 90, 91, 20, 1), (1, 130, 130, 36, 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("level,spread", [(1e5, 1.0), (1e6, 0.25), (1e8, 100.0), (-3e6, 1.0), (1e6, 0.0)])
+@pytest.mark.parametrize("shape", SLICED)
+def test_plane_in_slices_far_above_its_spread(shape, level, spread):
+    """Sums in f64 about the group's first value s: at most 2^13 roundings in a row, of sums that (s - mean)^2 <= N var keeps below
+    N + 1 times the variance, N < 2^20: 2^(13 + 20 - 53) = 2^-20 of 1/sigma, and the f32 steps behind it: 512 u holds.  x - mean
+    is exact (both lie within a factor of two) up to the mean's residue, which the kernel carries."""
+    B, H, W, C, G = shape
+    x = (level + spread * torch.randn(B, H, W, C, generator=torch.Generator().manual_seed(int(abs(level)) % 97))).to(DEV)
+    y, stats = gn.run_fwd(x, G, None, None, "none")
+    ref, mean, rstd, _, _ = gn.gn64(x.cpu(), G, None, None, "none")
+    got = stats.cpu().double()
+    assert float(((got[..., 1] - rstd).abs() / rstd).max()) <= 512 * U
+    assert float(((got[..., 0] - mean).abs() / mean.abs()).max()) <= 2 * U
+    assert float((y.cpu().double() - ref).abs().max()) <= 512 * U * max(1.0, float(ref.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,level,step", [(torch.float16, 4096.0, 4.0), (torch.float16, 60000.0, 32.0), (torch.bfloat16, 2.0 ** 20, 2.0 ** 13)])
+@pytest.mark.parametrize("every", [2, 1000, 100000])
+@pytest.mark.parametrize("shape", SLICED)
+def test_sixteen_bit_plane_of_two_neighbouring_values(shape, every, dtype, level, step):
+    """one value in `every` is one step of the type above the others: the sums are exact, and so is the variance up to the f64 steps
+    behind them"""
+    B, H, W, C, G = shape
+    x = torch.full((B * H * W * C,), level)
+    x[every // 2::every] += step
+    x = x.to(dtype).view(B, H, W, C).to(DEV)
+    assert x.unique().numel() == 2
+    y, stats = gn.run_fwd(x, G, None, None, "none")
+    ref, mean, rstd, _, _ = gn.gn64(x.cpu(), G, None, None, "none")
+    got = stats.cpu().double()
+    assert float(((got[..., 1] - rstd).abs() / rstd).max()) <= 4 * U
+    assert float(((got[..., 0] - mean).abs() / mean).max()) <= 2 * U
+    gn.check_fwd(x, G, None, None, "none", y, stats)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", gn.DTYPES)
+def test_first_value_that_is_not_finite(dtype, bad):
+    """the value that the sums are taken about: its group is NaN, its neighbours are what they were"""
+    x, _, _, _ = gn.make(2, 130, 130, 32, 2, dtype, seed=3)
+    clean, cs = gn.run_fwd(x, 2, None, None, "none")
+    x[1, 0, 0, 16] = bad
+    y, stats = gn.run_fwd(x, 2, None, None, "none")
+    assert bool(torch.isnan(y[1, ..., 16:]).all()) and bool(torch.isnan(stats[1, 1, 1]))
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[1, ..., :16], clean[1, ..., :16]) and torch.equal(stats[0], cs[0])
