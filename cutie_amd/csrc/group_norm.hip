@@ -370,23 +370,23 @@ __global__ __launch_bounds__(VEC > 1 ? 512 : 1024) void gn_bwd_resident(const ty
 }
 
 // dgamma[c] (+)= sum_b chan[b][c][0], dbeta[c] (+)= sum_b chan[b][c][1]: a workgroup owns 8 values, 32 lanes each add
-// every 32nd sample, the 32 sums are added in lane order
+// every 32nd sample, the 32 sums are added in lane order (f64: up to 65535 samples)
 __global__ __launch_bounds__(256) void gn_fold_params(const float* __restrict__ chan, int B, int C, float* __restrict__ dgamma,
                                                       float* __restrict__ dbeta, int accumulate) {
-    __shared__ float sh[32][8];
+    __shared__ double sh[32][8];
     const int el = threadIdx.x & 7, part = threadIdx.x >> 3;
     const int64_t i = (int64_t)blockIdx.x * 8 + el, n = (int64_t)C * 2;
-    float t = 0.f;
+    double t = 0;
     if (i < n)
         for (int b = part; b < B; b += 32) t += chan[b * n + i];
     sh[part][el] = t;
     __syncthreads();
     if (part || i >= n) return;
-    t = 0.f;
+    t = 0;
 #pragma unroll
     for (int k = 0; k < 32; ++k) t += sh[k][el];
     float* out = (i & 1) ? dbeta : dgamma;
-    if (out) out[i >> 1] = accumulate ? out[i >> 1] + t : t;
+    if (out) out[i >> 1] = (accumulate ? out[i >> 1] : 0.f) + (float)t;
 }
 
 // ------------------------------------------------------------------------------------------------------------------- split
@@ -415,18 +415,17 @@ template <int VEC> struct SplitMap {
     }
 };
 
+// slots[c][2] = the threads' sums in red, [2][thread][VEC], over the rows side by side
 template <int VEC, typename R>
-__device__ __forceinline__ void split_store(const R* a, const R* q, R (*red)[256 * VEC], const SplitMap<VEC>& m, int C, R* slots) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) { red[0][threadIdx.x * VEC + e] = a[e]; red[1][threadIdx.x * VEC + e] = q[e]; }
+__device__ __forceinline__ void split_store(const double (*red)[256 * VEC], const SplitMap<VEC>& m, int C, R* slots) {
     __syncthreads();
     const int n = m.nv * VEC;
     R* out = slots + ((m.b * gridDim.x + blockIdx.x) * C + (int64_t)blockIdx.z * 256 * VEC) * 2;
     for (int i = threadIdx.x; i < 2 * n; i += 256) {
         const int k = i / n, c = i - k * n;
-        R t = 0;
+        double t = 0;
         for (int r = 0; r < m.rows_par; ++r) t += red[k][r * n + c];
-        out[c * 2 + k] = t;
+        out[c * 2 + k] = (R)t;
     }
 }
 
@@ -462,7 +461,9 @@ __global__ __launch_bounds__(256) void gn_fwd_partial(const typename elem<DT>::t
             }
         }
     }
-    split_store<VEC>(a, q, red, m, C, slots);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { red[0][threadIdx.x * VEC + e] = a[e]; red[1][threadIdx.x * VEC + e] = q[e]; }
+    split_store<VEC>(red, m, C, slots);
 }
 
 // one workgroup per (group, sample): stats, and in `low` what the f32 mean misses
@@ -553,42 +554,64 @@ __device__ __forceinline__ void norms(Norm1* ch, const SplitMap<VEC>& m, int Cg,
     }
 }
 
+// f32 sums of GN_RUN pixels, which go to f64 sums in LDS: no chain of f32 additions is longer, however large the plane
+constexpr int GN_RUN = 64;
 template <int DT, int VEC>
 __global__ __launch_bounds__(256) void gn_bwd_partial(const typename elem<DT>::type* __restrict__ dy, int ld_dy,
                                                       const typename elem<DT>::type* __restrict__ x, int ld_x,
                                                       const float* __restrict__ gamma, const float* __restrict__ beta,
                                                       const float* __restrict__ stats, int act, int HW, int C, int G,
                                                       float* __restrict__ slots) {
-    __shared__ float red[2][256 * VEC];
+    __shared__ double red[2][256 * VEC];
     const SplitMap<VEC> m(HW, C);
     const int Cg = C / G;
-    float sx[VEC] = {}, sg[VEC] = {};
+    double *tx = red[0] + threadIdx.x * VEC, *tg = red[1] + threadIdx.x * VEC;      // this thread's sums of g * xhat and g
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) tx[e] = tg[e] = 0;
     if (m.on) {
         Norm1 ch[VEC];
         norms<VEC>(ch, m, Cg, G, stats, gamma, beta);
         with_act(act, [&](auto A) {
-#pragma unroll 2
-            for (int r = m.r0 + m.row; r < m.r1; r += m.rows_par) {
-                Pack<DT, VEC> vx, vd;
-                vx.load(x + (m.b * HW + r) * ld_x + m.c0);
-                vd.load(dy + (m.b * HW + r) * ld_dy + m.c0);
+            for (int r = m.r0 + m.row; r < m.r1;) {
+                const int stop = min(m.r1, r + GN_RUN * m.rows_par);
+                float sx[VEC] = {}, sg[VEC] = {};
+                auto fetch = [&](int at, Pack<DT, VEC>& vx, Pack<DT, VEC>& vd) {
+                    vx.load(x + (m.b * HW + at) * ld_x + m.c0);
+                    vd.load(dy + (m.b * HW + at) * ld_dy + m.c0);
+                };
+                auto add = [&](const Pack<DT, VEC>& vx, const Pack<DT, VEC>& vd) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float xe = vx.get(e), d = xe - ch[e].mean;
-                    const float g = vd.get(e) * act_grad<DT, decltype(A)::v>(xe, d, ch[e], gamma ? gamma + m.c0 + e : nullptr);
-                    sg[e] += g;
-                    sx[e] = fmaf(g, d, sx[e]);
+                    for (int e = 0; e < VEC; ++e) {
+                        const float xe = vx.get(e), d = xe - ch[e].mean;
+                        const float g = vd.get(e) * act_grad<DT, decltype(A)::v>(xe, d, ch[e], gamma ? gamma + m.c0 + e : nullptr);
+                        sg[e] += g;
+                        sx[e] = fmaf(g, d, sx[e]);
+                    }
+                };
+                Pack<DT, VEC> vx[2], vd[2];
+                // two pixels' loads together (one by one 512 x 512 x 1024 f32 takes 814 us, not 576)
+                for (; r + m.rows_par < stop; r += 2 * m.rows_par) {
+                    fetch(r, vx[0], vd[0]);
+                    fetch(r + m.rows_par, vx[1], vd[1]);
+                    add(vx[0], vd[0]);
+                    add(vx[1], vd[1]);
                 }
+                if (r < stop) {
+                    fetch(r, vx[0], vd[0]);
+                    add(vx[0], vd[0]);
+                    r += m.rows_par;
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) { tx[e] += (double)sx[e] * ch[e].rstd; tg[e] += sg[e]; }
             }
         });
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sx[e] *= ch[e].rstd;
     }
-    split_store<VEC>(sx, sg, red, m, C, slots);
+    split_store<VEC>(red, m, C, slots);
 }
 
 // one workgroup per (group, sample): chan[b][c][2] = the channel's sums over its slots (in slot order), and
-// grp[b][g][2] = (mean of h, mean of h * xhat)
+// grp[b][g][2] = (mean of h, mean of h * xhat).  At most 256 slots of a channel and 256 channels of a thread: f32 will do
+// (in f64 21 us in place of 12 for 4096 groups)
 __global__ __launch_bounds__(256) void gn_bwd_fold(const float* __restrict__ slots, int T, int HW, int C, int G,
                                                    const float* __restrict__ gamma, float* __restrict__ chan, float* __restrict__ grp) {
     __shared__ float red[2][256];

@@ -88,3 +88,36 @@ def test_first_value_that_is_not_finite(dtype, bad):
     y, stats = gn.run_fwd(x, 2, None, None, "none")
     assert bool(torch.isnan(y[1, ..., 16:]).all()) and bool(torch.isnan(stats[1, 1, 1]))
     assert torch.equal(y[0], clean[0]) and torch.equal(y[1, ..., :16], clean[1, ..., :16]) and torch.equal(stats[0], cs[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("HW,C,G,dtype", [((16384, 16384), 1, 1, torch.float32), ((4096, 4096), 24, 2, torch.bfloat16), ((512, 512), 1024, 32, torch.float32)])
+def test_backward_of_a_large_plane(HW, C, G, dtype):
+    """2^28 values of one channel, 4096 pixels a thread.  f32 sums are of 64 pixels; theirs are in f64, a slice's is rounded to f32
+    once, at most 256 slices of a channel are added in f32, in any order, and 16 more cover the terms' own roundings and a group's
+    channels: 336 u of the magnitudes.  (One f32 chain of 4096 equal terms of 0.7 drifts by 679.)  dy is one value, with a little
+    noise on half of the rows, so that roundings do not cancel."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn((1, *HW, C), generator=g, device=DEV).to(dtype)
+    dy = torch.full_like(x, 0.7)
+    dy[:, ::2] += 0.01 * torch.randn(dy[:, ::2].shape, generator=g, device=DEV).to(dtype)
+    y, stats = gn.run_fwd(x, G, None, None, "none")
+    del y
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(C, device=DEV), torch.empty(C, device=DEV)
+    ops.gn_bwd(dy, x, stats, dx, dgamma=dgamma, dbeta=dbeta)
+    n = HW[0] * HW[1]
+    half = gn.HALF[dtype]
+    for k in range(0, C, max(1, C // G)):      # group by group, f64 on the device
+        cut = slice(k, k + C // G)
+        mean, rstd = (stats[0, k // (C // G), i].double() for i in (0, 1))
+        xh = (x[0, ..., cut].double().reshape(n, -1) - mean) * rstd
+        d = dy[0, ..., cut].double().reshape(n, -1)
+        sg, sx, mg, mx = d.sum(0), (d * xh).sum(0), d.abs().sum(0), (d * xh).abs().sum(0)
+        assert bool(((dbeta[cut].double() - sg).abs() <= 336 * U * mg).all())
+        assert bool(((dgamma[cut].double() - sx).abs() <= 336 * U * mx).all())
+        N = n * (C // G)
+        ref = rstd * (d - sg.sum() / N - xh * (sx.sum() / N))
+        mag = rstd * (d.abs() + mg.sum() / N + xh.abs() * (mx.sum() / N))
+        err = (dx[0, ..., cut].double().reshape(n, -1) - ref).abs()
+        assert bool((err <= half * ref.abs() + 336 * U * mag).all()), float((err / (half * ref.abs() + 336 * U * mag)).max())
+        del xh, d, ref, mag, err
