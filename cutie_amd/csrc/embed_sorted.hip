@@ -506,12 +506,13 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const uint2* __restrict__ 
 
 // One workgroup per chunk (and JOIN vectors of columns): where a run starts in this chunk and leaves it (starts 1), the sum of its
 // parts up to the first chunk that it does not fill (starts 2: filled).  The parts go round the subgroups that a row of columns
-// leaves room for, whose sums are added in order.
+// leaves room for, whose sums are added in order.  In f64: a part is a sum of at most CHUNK_MAX rows in f32, but the parts of one id
+// are as many as the cells make (8388608 cells on one id, 516 columns: 8192 parts).
 constexpr int JOIN = 256;      // 131072 cells, most on one id: 9.3 us, 8.8 with 1024 threads; 500009 cells: 6.5 and 9.6
 template <int VEC>
 __global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict__ pairs, float* __restrict__ dtable, SumShape s,
                                                        const float* __restrict__ slots, const int* __restrict__ starts) {
-    __shared__ float sh[JOIN * VEC];
+    __shared__ double sh[JOIN * VEC];
     __shared__ int first;
     const int64_t w = blockIdx.x, tail = min(s.n, (w + 1) * s.rows * s.L) - 1;
     int64_t last = w + 1;
@@ -533,11 +534,14 @@ __global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict_
     }
     const int v0 = blockIdx.y * JOIN, nv = min(JOIN, s.E / VEC - v0), parts = JOIN / nv;
     const int col = threadIdx.x % nv, part = threadIdx.x / nv, c = (v0 + col) * VEC;
-    float t[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) t[e] = 0.f;
+    double t[VEC] = {};
     if (part < parts) {
-        if (part == 0) load_f32<VEC>(slots + (w * 2 + 1) * s.E + c, t);
+        if (part == 0) {
+            float v[VEC];
+            load_f32<VEC>(slots + (w * 2 + 1) * s.E + c, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) t[e] = v[e];
+        }
 #pragma unroll 8
         for (int64_t k = w + 1 + part; k <= last; k += parts) {
             float v[VEC];
@@ -554,7 +558,7 @@ __global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict_
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] += sh[(q * nv + col) * VEC + e];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) put(dtable, s, key, c + e, t[e]);
+    for (int e = 0; e < VEC; ++e) put(dtable, s, key, c + e, (float)t[e]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
