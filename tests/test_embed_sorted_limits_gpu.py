@@ -24,3 +24,47 @@ def test_parts_of_one_id_meet_in_f64():
     want = float(torch.tensor(1.3).double()) * n
     assert not got[0].any() and not got[2].any()
     assert float((got[1].double() - want).abs().max()) <= (1024 + 1 + 3) * U * want
+
+
+# rows that a workgroup takes one, two or more of, at every number of pairs a workgroup adds (64, 256, 1024), ids all one, most one
+WIDE = [
+    (300000, 3000, 512, "grid"), (300000, 3000, 512, "one"), (270000, 50, 1023, "grid"), (270000, 50, 1024, "one"), (270000, 50, 1024, "grid"),
+    (270000, 7, 516, "one"), (262144, 900, 260, "grid"), (65537, 40, 1032, "grid"), (65536, 40, 1032, "one"), (20000, 11, 4100, "grid"),
+    (5000, 3, 65536, "uniform"), (300000, 100000, 36, "uniform"), (300000, 300, 1, "grid"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", es.DTYPES)
+@pytest.mark.parametrize("n,V,E,kind", WIDE)
+def test_every_cell_counts_once(n, V, E, kind, dtype):
+    """whole-number rows of up to 31 either way, whose sums of any part stay below 2^24: every f32 sum is exact, and the result is
+    equal to the sum in whole numbers, scaled by a power of two"""
+    g = torch.Generator().manual_seed(n + V + E)
+    ids = es.draw_ids(n, V, kind, g).to(DEV)
+    gd = torch.Generator(device=DEV).manual_seed(E)
+    dout = torch.randint(-31, 32, (n, E), generator=gd, device=DEV, dtype=torch.int8).to(dtype)
+    want = torch.zeros(V, E, device=DEV)
+    for lo in range(0, n, 1 << 15):      # every addition is exact: the order is no matter
+        want.index_add_(0, ids[lo:lo + (1 << 15)].long(), dout[lo:lo + (1 << 15)].float())
+    assert float(want.abs().max()) < 2 ** 24
+    got = torch.full((V, E), 7.0, device=DEV)
+    ops.embed_grad_sorted(ids, dout, got, scale=0.25)
+    assert torch.equal(got, want * 0.25)
+    base = torch.randint(-99, 100, (V, E), generator=gd, device=DEV).float()
+    acc = base.clone()
+    ops.embed_grad_sorted(ids, dout, acc, scale=2.0, accumulate=True)
+    assert torch.equal(acc, base + want * 2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", es.DTYPES)
+@pytest.mark.parametrize("n,V,E,kind", [c for c in WIDE if c[0] * c[2] < 1.6e8])
+def test_rounded_sums(n, V, E, kind, dtype):
+    g = torch.Generator().manual_seed(n + V + E)
+    ids = es.draw_ids(n, V, kind, g)
+    dout = torch.randn(n, E, generator=torch.Generator(device=DEV).manual_seed(E), device=DEV).to(dtype)
+    got = torch.empty(V, E, device=DEV)
+    ops.embed_grad_sorted(ids.to(DEV), dout, got, scale=-1.5)
+    s, m = es.expect(ids, dout.cpu(), V, -1.5)
+    assert bool(((got.cpu().double() - s).abs() <= 1284 * U * m).all())

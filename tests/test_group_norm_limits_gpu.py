@@ -121,3 +121,47 @@ def test_backward_of_a_large_plane(HW, C, G, dtype):
         err = (dx[0, ..., cut].double().reshape(n, -1) - ref).abs()
         assert bool((err <= half * ref.abs() + 336 * U * mag).all()), float((err / (half * ref.abs() + 336 * U * mag)).max())
         del xh, d, ref, mag, err
+
+
+# batches of 256 (sample, group) pairs and more, whose workgroups take several groups of a pixel (their number in brackets, and the
+# threads side by side in a pixel): both kinds of sums, and samples that share a workgroup's share of groups with no other
+SEVERAL = [
+    (64, 16, 16, 64, 8),      # [2] 4 or 2 threads: lane exchanges
+    (64, 9, 7, 96, 8),        # [2] 6: through LDS
+    (64, 9, 7, 36, 12),       # [3] 9 single elements
+    (300, 5, 5, 40, 10),      # [10] 10
+    (128, 8, 8, 512, 64),     # [4 or 8] 8
+    (40, 31, 9, 264, 33),     # [3] 6 or 3
+    (512, 3, 3, 96, 4),       # [4] 24 or 12
+    (64, 16, 16, 192, 48),    # [4 or 8] vectors of four in a 16-bit type
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", gn.DTYPES)
+@pytest.mark.parametrize("act", ["silu", "relu"])
+@pytest.mark.parametrize("B,H,W,C,groups", SEVERAL)
+def test_several_groups_in_a_workgroup(B, H, W, C, groups, act, dtype):
+    check_both(B, H, W, C, groups, act, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", gn.DTYPES)
+@pytest.mark.parametrize("B,H,W,act", [(16, 64, 64, "silu"), (16, 48, 40, "sigmoid")])
+def test_the_widest_workgroups(B, H, W, act, dtype):
+    """256 channels in 32 groups, two of them a workgroup: 8 to 16 vectors a thread, 128 KB of x in LDS on the way back"""
+    check_both(B, H, W, 256, 32, act, dtype)
+
+
+def check_both(B, H, W, C, groups, act, dtype):
+    x, dy, gamma, beta = gn.make(B, H, W, C, groups, dtype, seed=B + C)
+    y, stats = gn.run_fwd(x, groups, gamma, beta, act)
+    gn.check_fwd(x, groups, gamma, beta, act, y, stats)
+    dx, dgamma, dbeta = torch.full_like(dy, 7.0), torch.full((C,), 7.0, device=DEV), torch.full((C,), 7.0, device=DEV)
+    ops.gn_bwd(dy, x, stats, dx, gamma=gamma, beta=beta, act=act, dgamma=dgamma, dbeta=dbeta)
+    gn.check_bwd(dy, x, stats, gamma, beta, act, dx, dgamma, dbeta)
+    # the whole batch is the samples one by one, which take another number of groups a workgroup: to the rounding of the sums
+    for b in (0, B - 1):
+        y1, s1 = gn.run_fwd(x[b:b + 1], groups, gamma, beta, act)
+        gn.check_fwd(x[b:b + 1], groups, gamma, beta, act, y1, s1)
+        assert float((s1[0] - stats[b]).abs().max()) <= 1024 * U * float(stats[b].abs().max() + 1)
