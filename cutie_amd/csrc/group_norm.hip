@@ -38,8 +38,9 @@ template <typename F> __device__ __forceinline__ void with_act(int act, F&& f) {
     }
 }
 
-// 1 / (1 + exp(-z)).  f32: the library's expf and divide.  16-bit outputs take the hardware exponential and reciprocal (a few units of 2^-23): half a
-// step of the output is 2^-11 (f16) or 2^-8 (bf16).
+// 1 / (1 + exp(-z)).  f32: the library's expf and divide.  The 16-bit types take the hardware exponential and reciprocal (a few units of
+// 2^-23, and |z| 2^-24 from the exponent's rounding): half a step of their outputs is 2^-11 (f16) or 2^-8 (bf16).  dgamma and dbeta are
+// f32 and are made of the same values, of gradients that came in 16 bits.
 template <int DT> __device__ __forceinline__ float sigmoid_of(float z) {
     if constexpr (DT == CUTIE_F32) return 1.f / (1.f + expf(-z));
     else return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
@@ -55,6 +56,7 @@ template <int DT, int A> __device__ __forceinline__ float act_of(float z) {
 // error of the gradient: where |z| is within the f32 error of its own computation (d = x - mean, a product and a sum: at
 // most 3 roundings, 2^-24 each, of |d * rg| + |beta|; 4e-7 > 3 * 2^-24) the sign is taken in f64.
 // gamma: the channel's, nullable (1).
+// mean is the stored f32 one: what it misses of the mean (up to 2^-24 of it) is in every xhat of the group.
 struct Norm1 { float mean, rstd, beta, rg; };      // of one channel; rg = rstd * gamma
 template <int DT, int A> __device__ __forceinline__ float act_grad(float x, float d, const Norm1& n, const float* gamma) {
     if constexpr (A == GN_ACT_NONE) return 1.f;

@@ -498,7 +498,7 @@ def gn_fwd(x, y, stats, gamma=None, beta=None, act=None, eps=GN_EPS, workspace=N
 
 
 def gn_bwd(dy, x, stats, dx, gamma=None, beta=None, act=None, dgamma=None, dbeta=None, accumulate=False, workspace=None):
-    """Gradient of gn_fwd (cutie_gn_bwd): x and stats of the forward, the same gamma / beta / act; dx [B,H,W,C] view; dgamma,
+    """Gradient of gn_fwd (cutie_gn_bwd) at the statistics as they are stored: x and stats of the forward, the same gamma / beta / act; dx [B,H,W,C] view; dgamma,
     dbeta f32 [C] or None, overwritten or (accumulate) added to.  Returns dx."""
     B, HW, C = _gn_views("gn_bwd", x, stats, act, (dy, dx))
     need = gn_workspace_bytes(B, HW, C, stats.shape[1])

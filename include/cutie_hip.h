@@ -360,8 +360,12 @@ int cutie_spatial_mean_bcast(const void* x, int ld_x, int x_dtype, void* out, in
  *        dgamma[c] = sum g * xhat, dbeta[c] = sum g over (b, hw)  (each nullable; accumulate != 0 adds to what is there)
  * gamma / beta f32 [C], each nullable (1 and 0).  x, y, dy, dx share one dtype, any channel count that `groups` divides, any
  * leading dimension >= C; groups of 16 bytes or a multiple of them move fastest, in views whose base and leading dimension are such.
- * An output may not overlap an input (slices of one wide buffer are fine).  Sums are f32 or f64 in a fixed order: reruns are bit-identical.  A value next to the
- * step of the ReLU takes the side that f64 arithmetic on (x, stats, gamma, beta) gives.  B, C, groups <= 65535, eps > 0.
+ * An output or the workspace may not overlap another tensor of the call (slices of one wide buffer are fine).  Sums are f32 or f64
+ * in a fixed order: reruns are bit-identical.  A value next to the step of the ReLU takes the side that f64 arithmetic on (x, stats,
+ * gamma, beta) gives.  The backward takes the statistics as they are stored: the f32 mean is off by up to 2^-24 of itself, so every
+ * xhat of a group by up to 2^-24 |mean| * rstd (2.4e-4 at a level of 4096 sigma); the forward carries what its mean misses.
+ * Sigmoid and SiLU of the 16-bit types take the hardware's exponential and reciprocal (a few 2^-23 of the sigmoid, and |z| 2^-24 more),
+ * also behind the f32 outputs dgamma and dbeta; f32 takes the library's.  B, C, groups <= 65535, HW <= 2^30, eps > 0.
  * workspace: cutie_gn_workspace_bytes(B, HW, C, groups) bytes, 16-byte aligned, clobbered, no pre-fill.  B = 0 or HW = 0
  * stores no activations; dgamma and dbeta are then cleared (accumulate == 0) or left alone. */
 #define CUTIE_ACT_SILU 3

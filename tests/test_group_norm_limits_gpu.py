@@ -165,3 +165,35 @@ def check_both(B, H, W, C, groups, act, dtype):
         y1, s1 = gn.run_fwd(x[b:b + 1], groups, gamma, beta, act)
         gn.check_fwd(x[b:b + 1], groups, gamma, beta, act, y1, s1)
         assert float((s1[0] - stats[b]).abs().max()) <= 1024 * U * float(stats[b].abs().max() + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("shape", [(1, 16, 16, 32, 4), (1, 130, 130, 32, 2)])
+def test_backward_at_a_level_far_above_the_spread(shape, act):
+    """against the gradient at the values' own statistics.  The backward takes the mean as it is stored, rounded to f32: every xhat is
+    off by one r <= 2^-24 |mean| / sigma (2.4e-4 here: 4096 sigma), and with it dgamma by r sum |g|, and dx by what r moves in
+    xhat mean(h xhat) and, through act'' (at most 1/2), in h.  Nothing else is lost to the level."""
+    B, H, W, C, G = shape
+    g = torch.Generator().manual_seed(4)
+    x = (4096.0 + torch.randn(B, H, W, C, generator=g)).to(DEV)
+    dy = torch.randn(B, H, W, C, generator=g).to(DEV)
+    gamma, beta = (1 + 0.3 * torch.randn(C, generator=g)).to(DEV), (0.3 * torch.randn(C, generator=g)).to(DEV)
+    _, stats = gn.run_fwd(x, G, gamma, beta, act)
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty(C, device=DEV), torch.empty(C, device=DEV)
+    ops.gn_bwd(dy, x, stats, dx, gamma=gamma, beta=beta, act=act, dgamma=dgamma, dbeta=dbeta)
+    _, mean, rstd, xh, z = gn.gn64(x.cpu(), G, gamma.cpu(), beta.cpu(), act)
+    true = torch.stack([mean, rstd], dim=-1)
+    ref, rg, rb, mag, mg, mb = gn.gn_bwd64(dy.cpu(), x.cpu(), true, gamma.cpu(), beta.cpu(), act)
+    r = 2.0 ** -24 * float((mean.abs() * rstd).max())
+    ga, d = gamma.cpu().double(), dy.cpu().double().abs()
+    dh = 0.5 * r * d * ga ** 2 if act == "silu" else torch.zeros_like(d)      # h may be off by this
+    grouped = lambda t: t.reshape(B, H * W, G, C // G)
+    mean_of = lambda t: grouped(t).mean((1, 3), keepdim=True).expand(B, H * W, G, C // G).reshape(B, H, W, C)
+    h = (1.1 * d * ga.abs())      # |act'| <= 1.1
+    rs = rstd.reshape(B, 1, G, 1).expand(B, H * W, G, C // G).reshape(B, H, W, C)
+    tol = 512 * U * mag + rs * (dh + mean_of(dh) + xh.abs() * mean_of(dh * xh.abs()) + 2 * r * (mean_of(h * xh.abs()) + xh.abs() * mean_of(h)))
+    assert bool(((dx.cpu().double() - ref).abs() <= U * ref.abs() + tol).all())
+    sg = (dh / ga.abs()).sum((0, 1, 2))
+    assert bool(((dbeta.cpu().double() - rb).abs() <= 512 * U * mb + sg).all())
+    assert bool(((dgamma.cpu().double() - rg).abs() <= 512 * U * mg + (dh / ga.abs() * xh.abs()).sum((0, 1, 2)) + 1.1 * r * d.sum((0, 1, 2)) + r * sg).all())
