@@ -498,8 +498,8 @@ def gn_fwd(x, y, stats, gamma=None, beta=None, act=None, eps=GN_EPS, workspace=N
 
 
 def gn_bwd(dy, x, stats, dx, gamma=None, beta=None, act=None, dgamma=None, dbeta=None, accumulate=False, workspace=None):
-    """Gradient of gn_fwd (cutie_gn_bwd) at the statistics as they are stored: x and stats of the forward, the same gamma / beta / act; dx [B,H,W,C] view; dgamma,
-    dbeta f32 [C] or None, overwritten or (accumulate) added to.  Returns dx."""
+    """Gradient of gn_fwd (cutie_gn_bwd) at the statistics as they are stored: x and stats of the forward, the same gamma / beta /
+    act; dx [B,H,W,C] view; dgamma, dbeta f32 [C] or None, overwritten or (accumulate) added to.  Returns dx."""
     B, HW, C = _gn_views("gn_bwd", x, stats, act, (dy, dx))
     need = gn_workspace_bytes(B, HW, C, stats.shape[1])
     ws = _workspace(workspace, need, x.device, "gn_bwd")
@@ -755,7 +755,9 @@ def muon_step(entries, lr, momentum=0.95, nesterov=True, weight_decay=0.0, l2=0.
     returned.  gnorm_sq: f32 [1] squared global norm on the device, for the clip and to skip a step that is not finite;
     loss_scale: the K12 state; invalid: int32 [1], non-zero skips the step.  workspace: optional uint8 tensor of
     orthogonalize_workspace_bytes(shapes) bytes."""
-    arr, shapes, device = entries if isinstance(entries, tuple) else muon_descs(entries)
+    # a plan ends in its device; matrices may come as a tuple as well as in a list
+    plan = isinstance(entries, tuple) and len(entries) == 3 and isinstance(entries[2], torch.device)
+    arr, shapes, device = entries if plan else muon_descs(entries)
     ws = _orth_space(shapes, device, workspace, "muon_step")
     for t, what, dt, n in ((gnorm_sq, "gnorm_sq", torch.float32, 1), (loss_scale, "loss_scale", torch.float32, 2),
                            (invalid, "invalid", torch.int32, 1)):
