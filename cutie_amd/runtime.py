@@ -42,6 +42,14 @@ def _scale(node):
     return node.attrs.get("scale", 1.0)
 
 
+def check_muon(hp, clip):
+    """refuses, before anything is updated, what cutie_muon_step would refuse behind the Adam pass of the same step"""
+    if not 1 <= hp["steps"] <= 32:
+        raise ValueError("%r steps of the orthogonalised update (1..32)" % (hp["steps"],))
+    if not clip > 0:
+        raise ValueError("clip norm %r: the orthogonalised update takes Adam's clipped gradient, which needs a positive one" % (clip,))
+
+
 class _Plan(object):
     pass
 
@@ -806,6 +814,8 @@ class Engine(object):
         Returns the 1-float device tensor of the squared global norm (of the summed gradient)."""
         if not getattr(P, "raw_grads", False):
             raise CutieError("apply_update needs loss_backward(..., defer_l2=True)")
+        if muon is not None:
+            check_muon(muon, clip)
         wd = float(self.net.loss_spec["weight_decay"])
         # which conv kernels Adam takes: all of them, or the logits layer's alone (Trainer keeps to one of the two)
         if getattr(self, "_opt_layers", None) is None or self._opt_muon != (muon is not None):

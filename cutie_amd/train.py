@@ -16,6 +16,7 @@ import os
 import torch
 
 from .parallel import GradBuckets, dist_info
+from .runtime import check_muon
 
 
 class Trainer(object):
@@ -34,6 +35,7 @@ class Trainer(object):
         if optimizer == "muon":
             self.muon = {"lr": float(muon_lr), "momentum": float(muon_momentum), "nesterov": bool(muon_nesterov),
                          "weight_decay": float(muon_weight_decay), "steps": int(muon_steps)}
+            check_muon(self.muon, clip_norm)
         self.clip, self.b1, self.b2, self.eps = float(clip_norm), beta1, beta2, epsilon
         self.lr_decay_step, self.lr_decay_factor = lr_decay_step, lr_decay_factor
         self.iter = 0          # the reference's `iter` (drives lr decay)
