@@ -122,3 +122,15 @@ def test_update_of_a_large_matrix():
     want = p0.double() * (1 - 0.02 * 0.01) - 0.02 * 1.25 * x
     tol = 0.02 * 1.25 * off + 4 * mu.U * (float(p0.double().norm()) + 0.02 * 1.25 * float(x.norm()))
     assert float((p.double() - want).norm()) <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["normal", "rank1"])
+@pytest.mark.parametrize("r,c", [(1 << 20, 1), (5, 100001), (8193, 64), (30001, 70)])
+def test_long_and_thin(r, c, kind):
+    """more rows than the form with one launch a step takes"""
+    u = mu.matrix(r, c, kind, torch.Generator().manual_seed(r + c)).to(DEV)
+    out = torch.full_like(u, 7.0)
+    ops.orthogonalize_batched([(u, out)])
+    want, tol = allowed(u)
+    assert float((out.double() - want).norm()) <= tol
