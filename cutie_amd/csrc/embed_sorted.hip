@@ -5,8 +5,9 @@
 //
 // Measured (MI355X), inputs that change from call to call: lookup 131072 x 128 f16 9 us, 500009 x 512 bf16 187 us (4.1 TB/s of the
 // 760 MB it must move; 156 us on the same inputs again); gradient 131072 x 128 f16, V 18000, 94 % of the cells on one id: 49 us in six
-// launches (27 us the two passes of the sort, 15 the sums, 9 the join); 500009 x 512 bf16, V 120000: 227 us, of which the sums 155
-// (4.9 TB/s).
+// launches (27 us the two passes of the sort, 15 the sums, 8 the join); 500009 x 512 bf16, V 120000: 228 us, of which the sums 155
+// (4.9 TB/s of the 760 MB).  The gradient by float atomics of embed.hip is faster on the first - back to back on one input 21 us
+// against 46 - in an order of its own every run; a train step of CUTIE-ASPP on 32 documents has 7.55 ms with it, 7.56 with this one.
 //
 // The lookup is a row copy (HBM).  The gradient sorts (id, cell) pairs - a stable radix sort, least significant digit
 // first - and adds runs of equal ids: every output row has one owner, no float atomics, the same bits every run, and an id
@@ -508,7 +509,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const uint2* __restrict__ 
 // parts up to the first chunk that it does not fill (starts 2: filled).  The parts go round the subgroups that a row of columns
 // leaves room for, whose sums are added in order.  In f64: a part is a sum of at most CHUNK_MAX rows in f32, but the parts of one id
 // are as many as the cells make (8388608 cells on one id, 516 columns: 8192 parts).
-constexpr int JOIN = 256;      // 131072 cells, most on one id: 9.3 us, 8.8 with 1024 threads; 500009 cells: 6.5 and 9.6
+constexpr int JOIN = 256;      // 131072 cells, most on one id: 9.3 us, 8.8 with 1024 threads; 500009 cells: 6.5 and 9.6 (sums in f32)
 template <int VEC>
 __global__ __launch_bounds__(JOIN) void run_join_kernel(const uint2* __restrict__ pairs, float* __restrict__ dtable, SumShape s,
                                                        const float* __restrict__ slots, const int* __restrict__ starts) {

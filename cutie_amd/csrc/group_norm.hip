@@ -13,8 +13,8 @@
 // fold, and a second pass over the operands.
 //
 // Measured (MI355X), 32 x 64 x 64 x 256, 32 groups (134 MB forward, 201 MB backward), inputs that change from call to call: forward
-// f16 33 us resident (4.1 TB/s), backward bf16 SiLU 73 us + 5 us fold (2.6 TB/s).  The same inputs again, partly in cache: 30 and
-// 54 + 5 us; split form 50 and 86.  What decides is the width of the piece of a pixel that a workgroup reads (its groups'
+// f16 33 us resident (4.1 TB/s), backward bf16 SiLU 73 us + 5 us fold (2.6 TB/s).  The same inputs again, partly in cache: 32 and
+// 54 us with the fold, f32 61 and 136 (268 and 403 MB); split form 50 and 86.  What decides is the width of the piece of a pixel that a workgroup reads (its groups'
 // channels): 16 bytes 50 us forward, 32 bytes 31, 64 bytes 30 - L2 hands out 64 bytes at least - and, backward, one exponential
 // and one reciprocal an element instead of two (86 us when the store pass made g again).  Non-temporal stores: 38 and 90 us
 // (pieces of a line no longer meet in L2).  The backward keeps 128 KB of x in LDS, so a CU holds one workgroup and its loads wait
@@ -728,7 +728,7 @@ inline int gn_vec(int dt, int run) {
 }
 
 // of the split form, whose threads carry their channels' constants: four (8 x 128 x 128 x 64 f16 29 us backward, eight 35, single elements
-// 32), eight of a wide row (512 x 512 x 1024: 622 us, four 713)
+// 32), eight of a wide row (512 x 512 x 1024 bf16: 622 us, four 713; with the sums of two pixels at a time 611)
 inline int gn_split_vec(int dt, int C) {
     const int v = gn_vec(dt, C);
     return v == 8 && C < 1024 ? 4 : v;

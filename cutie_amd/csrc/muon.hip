@@ -17,8 +17,10 @@
 // a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
 // of a product is one 128-byte line of a row.  A and B [S][S] alike.
 //
-// Measured (MI355X), five steps: 14 filters (10 of them 3840 x 256) 411 - 428 us, of which the matrix cores need 110 for the three
-// products at the rate of a large library product; 2048 x 8192 1.84 ms (1.45 ms likewise; in f32 the library's rate gives 3.6).
+// Measured (MI355X), five steps, calls back to back on one input, all on one box - the figures of this file are of this kind: 14 filters
+// (10 of them 3840 x 256) 355 us, of which the matrix cores need 110 for the three products at the rate of a large library product;
+// 2048 x 8192 1.75 ms (1.45 ms likewise; in f32 the library's rate gives 3.6).  One call among others, on inputs that change, the
+// update of the 14 filters takes 410 - 451 us, 2048 x 8192 1.77 - 1.91 ms, by the box.
 // There are three forms: the general one of this comment, and two for fewer columns, in f32, below.
 #include "conv_common.h"
 
@@ -210,7 +212,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Mats ms, Ios ios, Starts 
 // 128-byte lines (hi and lo) go to LDS by buffer_load ... lds, STAGES of them, all but one in flight while that one is used.
 template <int F> struct Shape {
     static constexpr int T = 32 * F, HALF = T * 128, STAGE = 2 * HALF;      // bytes of one operand, of both
-    // F = 4: two workgroups a CU with two stages (14 filters 458 us, 2048 x 8192 1.84 ms) beat one with three (535 us, 2.29 ms).
+    // F = 4: two workgroups a CU with two stages (14 filters 355 us, 2048 x 8192 1.75 ms) beat one with three (403 us, 2.27 ms).
     // F = 2: two, three and four stages are alike.
     static constexpr int STAGES = F == 4 ? 2 : 3;
     static constexpr int LDS = STAGES * STAGE;
@@ -498,8 +500,8 @@ template <int F, bool LAST, bool MUON>
 __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Starts st, Hyper h, int which, char* ws) {
     typedef Shape<F> S;
     __shared__ __attribute__((aligned(1024))) char smem[S::LDS];
-    // block order as dispatched: an XCD's workgroups share one or two column tiles of B, which stay in its L2, and stream X (183 us
-    // at 2048 x 8192; with an XCD's blocks consecutive 205)
+    // block order as dispatched: an XCD's workgroups share one or two column tiles of B, which stay in its L2, and stream X (2048 x 8192
+    // 1.75 ms, with an XCD's blocks consecutive 1.86; 14 filters 355 us and 350)
     const int i = find(st, ms.n, blockIdx.x);
     const Mat M = ms.m[i];
     const int nt = (M.Sp + S::T - 1) / S::T, id = blockIdx.x - st.v[i];
@@ -560,8 +562,8 @@ __global__ __launch_bounds__(256, 2) void ns_apply_kernel(Mats ms, Ios ios, Star
 // ------------------------------------------------------------------------------------------------------------------- small
 // Matrices of few rows and columns: one workgroup does everything, X, A and B as f32 in LDS, the products on the f32 matrix cores
 // (16 x 16 x 4; they have a sixteenth of the f16 rate, but the launches of the general form alone take longer).  The limit is where
-// the tall form below takes as long.  Five steps, one matrix: 128 x 16 17 us (tall 36), 352 x 16 35 (39), 64 x 18 18,
-// 288 x 32 48 (42), 192 x 48 61 (53), 128 x 64 56 (66), 192 x 64 80 (67).
+// the tall form below takes as long.  Five steps, one matrix: 128 x 16 16 us (tall 29, general 76), 352 x 16 35 (32), 64 x 18 17,
+// 288 x 32 48 (36), 192 x 48 61 (48), 128 x 64 55 (63), 192 x 64 80 (64).
 constexpr int SMALL_S = 64, SMALL_THREADS = 512, SMALL_WAVES = SMALL_THREADS / 64;
 constexpr int TALL_L = 8192;
 __host__ __device__ inline int up16(int v) { return (v + 15) & ~15; }
@@ -704,7 +706,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(Smalls sm, Ios 
 // S <= SMALL_S and L <= TALL_L: tiles of rows, one workgroup each, f32 products as above.  The first launch makes U and each
 // tile's part of U^T U; a step is one launch, in which every workgroup adds up all parts of A, makes B, takes its rows of X through
 // it and, for the step after, makes its part of X'^T X': 1 + steps launches in place of the general form's 2 + 4 steps.
-// One matrix, five steps: 3 x 3552 45 us (general form 112), 1024 x 64 73 (120), 5634 x 42 87 (163), 8192 x 64 136 (187), of which
+// One matrix, five steps: 3 x 3552 39 us (general form 111), 1024 x 64 70 (89), 5634 x 42 84 (144), 8192 x 64 134 (173), of which
 // the launches alone take 30.  At S = 64 the rest is the f32 matrix cores and, with 32 tiles, each workgroup's 512 KB of parts.
 constexpr int TALL_TILES = 32, TALL_ROWS = 64;
 struct Tall { int rows, cols, R, tiles, y, slab, head; };      // y [tiles R][S], slab [2][tiles][S][S], head [tiles]
@@ -865,8 +867,8 @@ __global__ __launch_bounds__(T) void ns_tall_step_kernel(Talls ts, Ios ios, Star
 
 // ------------------------------------------------------------------------------------------------------------------- host
 // All matrices of a call are computed in one form, the cheapest that takes every one of them: a matrix more in a form's launches costs
-// little, the launches of a second form come on top (14 filters of which one is 7680 x 64 and one 64 x 18: 458 us; with those two in
-// launches of their own forms 575).
+// little, the launches of a second form come on top (14 filters of which one is 7680 x 64 and one 64 x 18: 355 us; the twelve others
+// 329, those two in launches of their own forms 128 and 17 more).
 struct NsPlan {
     enum { SMALL, TALL, GENERAL } form;
     Mats ms;                 // GENERAL
@@ -902,8 +904,8 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
         else if (p.form == NsPlan::SMALL && !is_small(r, c)) p.form = NsPlan::TALL;
         if (S > 48) broad += cdiv(L, tall_rows(L));
     }
-    // One round of workgroups: at S = 64 the f32 products of more take longer than the general form (8192 x 64: 4 matrices 151 us,
-    // general 231; 32 matrices 711, general 453.  At S = 48 32 of 7079 x 35 take 343, general 478)
+    // One round of workgroups: at S = 64 the f32 products of more take longer than the general form (8192 x 64: 4 matrices 149 us,
+    // general 223; 32 matrices 708, general 425.  At S = 48 32 of 7079 x 35 take 333, general 340)
     if (p.form == NsPlan::TALL && broad > 256) p.form = NsPlan::GENERAL;
     size_t off = 0;      // of the workspace, in units of 256 bytes
     auto take = [&](int64_t bytes) {
@@ -950,10 +952,11 @@ inline int ns_plan(const char* who, const int* shapes, int n, NsPlan& p) {
         m.Lp = (int)Lp;
         m.Sp = (int)Sp;
     }
-    // X B and A A: the 128 tile where it gives every CU a workgroup (A A: with K cut into pieces of eight steps; 14 filters 458 us,
-    // with the 64 tile for X B 486; 2048 x 8192 1.84 ms, 2.49).  X^T X: where it gives each four (2048 x 8192 1.84 ms, 64 tile 2.14;
-    // 32 of 3840 x 256 832 us, 898), else the 64 tile, which wastes less of the diagonal's tiles (14 filters 428 us, 128 tile 458;
-    // two of 4608 x 512 306, 345).  K is cut for two workgroups a CU (512 / tiles; 256 / tiles 2.25 ms, 1024 / tiles for 14 filters 496 us)
+    // X B and A A: the 128 tile where it gives every CU a workgroup (A A: with K cut into pieces of eight steps; 14 filters 355 us,
+    // with the 64 tile for X B 397; 2048 x 8192 1.75 ms, 2.46).  X^T X: where it gives each four (2048 x 8192 1.75 ms, 64 tile 2.05;
+    // 32 of 3840 x 256 789 us, 870), else the 64 tile, which wastes less of the diagonal's tiles (14 filters 355 us, 128 tile 379;
+    // two of 4608 x 512 296, 337).  K is cut for two workgroups a CU (512 / tiles: 14 filters 355 us, 2048 x 8192 1.75 ms, 32 of
+    // 3840 x 256 789 us; 256 / tiles 429, 2.14, 861; 1024 / tiles 349, 1.77, 843)
     int64_t tg = 0, ts = 0, ta = 0;
     for (int i = 0; i < n; ++i) {
         const Mat& m = p.ms.m[i];
@@ -1051,8 +1054,8 @@ inline int ns_run(const NsPlan& p, const Ios& ios, const Hyper& h, int steps, fl
             wgs += p.tall.t[i].tiles;
         }
         st.v[p.tall.n] = wgs;
-        // 16 waves where a workgroup has a CU to itself and its products are long enough for them (5634 x 42: 88 us, 8 waves 107;
-        // 32 of 7079 x 35: 430 us, 8 waves 343; 11 x 5496: 60, 8 waves 50)
+        // 16 waves where a workgroup has a CU to itself and its products are long enough for them (5634 x 42: 84 us, 8 waves 104;
+        // 32 of 7079 x 35: 401 us, 8 waves 333; 11 x 5496: 49, 8 waves 46)
         return p.tall_wide && wgs <= 256 ? ns_tall<1024, MUON>(p, ios, st, h, wgs, steps, eps, ws, stream)
                                          : ns_tall<512, MUON>(p, ios, st, h, wgs, steps, eps, ws, stream);
     }
