@@ -14,10 +14,10 @@
 //
 // Measured (MI355X), 32 x 64 x 64 x 256, 32 groups (134 MB forward, 201 MB backward), inputs that change from call to call: forward
 // f16 33 us resident (4.1 TB/s), backward bf16 SiLU 73 us + 5 us fold (2.6 TB/s).  The same inputs again, partly in cache: 32 and
-// 54 us with the fold, f32 61 and 136 (268 and 403 MB); split form 50 and 86.  What decides is the width of the piece of a pixel that a workgroup reads (its groups'
-// channels): 16 bytes 50 us forward, 32 bytes 31, 64 bytes 30 - L2 hands out 64 bytes at least - and, backward, one exponential
-// and one reciprocal an element instead of two (86 us when the store pass made g again).  Non-temporal stores: 38 and 90 us
-// (pieces of a line no longer meet in L2).  The backward keeps 128 KB of x in LDS, so a CU holds one workgroup and its loads wait
+// 54 us with the fold, f32 61 and 136 (268 and 403 MB); split form 50 and 86.  What decides is the width of the piece of a pixel
+// that a workgroup reads (its groups' channels): 16 bytes 50 us forward, 32 bytes 31, 64 bytes 30 - L2 hands out 64 bytes at least -
+// and, backward, one exponential and one reciprocal an element instead of two (86 us when the store pass made g again).
+// Non-temporal stores: 38 and 90 us (pieces of a line no longer meet in L2).  The backward keeps 128 KB of x in LDS, so a CU holds one workgroup and its loads wait
 // while it makes its sums.  One document (B = 1): 12 us on 32 CUs, the latency of a load, two sums and 4 us of arithmetic.
 #include "common.h"
 

@@ -17,10 +17,10 @@
 // a wide matrix is made when it is normalised); a row is blocks of 32 values, 64 bytes hi and 64 bytes lo, so that one K step
 // of a product is one 128-byte line of a row.  A and B [S][S] alike.
 //
-// Measured (MI355X), five steps, calls back to back on one input, all on one box - the figures of this file are of this kind: 14 filters
+// Measured (MI355X), five steps, calls back to back on one input, all on one GPU - the figures of this file are of this kind: 14 filters
 // (10 of them 3840 x 256) 355 us, of which the matrix cores need 110 for the three products at the rate of a large library product;
 // 2048 x 8192 1.75 ms (1.45 ms likewise; in f32 the library's rate gives 3.6).  One call among others, on inputs that change, the
-// update of the 14 filters takes 410 - 451 us, 2048 x 8192 1.77 - 1.91 ms, by the box.
+// update of the 14 filters takes 410 - 451 us, 2048 x 8192 1.77 - 1.91 ms, by the GPU.
 // There are three forms: the general one of this comment, and two for fewer columns, in f32, below.
 #include "conv_common.h"
 
