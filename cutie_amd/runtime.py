@@ -280,6 +280,7 @@ class Engine(object):
         P.labels_buf = torch.zeros((B, H, W), dtype=torch.int32, device=dev)
         P.grid, P.labels = P.grid_buf, P.labels_buf      # forward() points them at the caller's device tensors where it can
         P.ps = torch.zeros((B, H * W), dtype=torch.int32, device=dev) if Hi else None
+        P.embed_rows = []      # (gradient of the looked-up rows, factor of the rows) of every embedding, by loss_backward
         P.bwd_ready = False
         self._plans[key] = P
         return P
@@ -695,7 +696,7 @@ class Engine(object):
         defer = self.wgrad_batch and side is None
         pending = []
         pending_elems = [0]
-        P.embed_rows = []      # (gradient of the looked-up rows, factor of the rows) of every embedding
+        P.embed_rows = []
 
         def flush():
             if not pending:

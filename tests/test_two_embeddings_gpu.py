@@ -74,3 +74,11 @@ def test_gradients_and_norm(large, small, embed_grad, dtype, gtol):
     m, v = torch.zeros_like(eng.params_flat), torch.zeros_like(eng.params_flat)
     assert abs(float(eng.apply_update(P, m, v, 1e-3, 0.9, 0.999, 1e-8, 1.0, t=1)) - want) < 2 * gtol * want
     assert not eng.grads_flat[eng.n_dense:].any()      # cleared behind itself, both tables
+
+
+@pytest.mark.gpu
+def test_before_any_backward_pass_the_rows_count_nothing():
+    eng = base.engine(TwoNet((V, 64, 1.0), (V, 64, 2.0)), "f16")
+    grid, labels = base.inputs(9)
+    P = eng.forward(grid, labels=labels)
+    assert float(eng.embedding_rows_sumsq(P)) == 0.0
