@@ -68,3 +68,21 @@ def test_rounded_sums(n, V, E, kind, dtype):
     ops.embed_grad_sorted(ids.to(DEV), dout, got, scale=-1.5)
     s, m = es.expect(ids, dout.cpu(), V, -1.5)
     assert bool(((got.cpu().double() - s).abs() <= 1284 * U * m).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,E", [(torch.float16, 516), (torch.float32, 513)])
+def test_lookup_beyond_32_bits_of_values(dtype, E):
+    n, V = (1 << 23) + 5, 77
+    g = torch.Generator(device=DEV).manual_seed(3)
+    ids = torch.randint(-1, V, (n,), generator=g, device=DEV, dtype=torch.int32)
+    table = torch.randn(V, E, generator=g, device=DEV)
+    out = torch.empty((n, E), dtype=dtype, device=DEV)
+    assert out.numel() > 2 ** 32
+    oob = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.embed_scaled_fwd(ids, table, out, 1.5, oob)
+    assert int(oob) == int((ids < 0).sum())
+    rows = torch.cat([table * 1.5, torch.zeros(1, E, device=DEV)]).to(dtype)      # an id outside the table: a row of zeros
+    for lo in range(0, n, 1 << 20):
+        i = ids[lo:lo + (1 << 20)].long()
+        assert torch.equal(out[lo:lo + (1 << 20)], rows[torch.where(i < 0, V, i)]), lo

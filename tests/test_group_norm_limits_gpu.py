@@ -197,3 +197,34 @@ def test_backward_at_a_level_far_above_the_spread(shape, act):
     sg = (dh / ga.abs()).sum((0, 1, 2))
     assert bool(((dbeta.cpu().double() - rb).abs() <= 512 * U * mb + sg).all())
     assert bool(((dgamma.cpu().double() - rg).abs() <= 512 * U * mg + (dh / ga.abs() * xh.abs()).sum((0, 1, 2)) + 1.1 * r * d.sum((0, 1, 2)) + r * sg).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,W,C,groups", [
+    (17000, 32, 32, 256, 32),      # whole groups in a workgroup
+    (3, 8192, 8192, 24, 2),        # in slices
+])
+def test_offsets_beyond_32_bits(B, H, W, C, groups):
+    """more than 2^32 values: the last sample alone, as a view of the same memory, gives the same bits or, where a batch takes another
+    number of groups a workgroup, the same values to the rounding of the sums"""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.empty((B, H, W, C), dtype=torch.bfloat16, device=DEV)
+    assert x.numel() > 2 ** 32
+    step = max(1, B // 16)
+    for lo in range(0, B, step):
+        x[lo:lo + step] = torch.randn(x[lo:lo + step].shape, generator=g, device=DEV, dtype=torch.bfloat16)
+    dy = torch.flip(x, dims=(0,))
+    y, stats, dx = torch.empty_like(x), torch.empty(B, groups, 2, device=DEV), torch.empty_like(x)
+    dgamma, dbeta = torch.empty(C, device=DEV), torch.empty(C, device=DEV)
+    ops.gn_fwd(x, y, stats, act="silu")
+    ops.gn_bwd(dy, x, stats, dx, act="silu", dgamma=dgamma, dbeta=dbeta)
+    for b in (0, B - 1):
+        y1, s1, dx1 = torch.empty_like(x[b:b + 1]), torch.empty(1, groups, 2, device=DEV), torch.empty_like(x[b:b + 1])
+        ops.gn_fwd(x[b:b + 1], y1, s1, act="silu")
+        assert float((s1[0] - stats[b]).abs().max()) <= 1024 * U * float(stats[b].abs().max() + 1)
+        ops.gn_bwd(dy[b:b + 1], x[b:b + 1], stats[b:b + 1].contiguous(), dx1, act="silu")
+        # two roundings to bf16 of values that agree to f32 rounding: equal, or neighbours
+        for got, want in ((y[b], y1[0]), (dx[b], dx1[0])):
+            assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+            assert float((got != want).float().mean()) < 1e-3
+    assert bool(torch.isfinite(dgamma).all()) and bool(torch.isfinite(dbeta).all())
